@@ -1,5 +1,5 @@
-// Shared pieces of libb200q: the ggml IQ2_XXS tables, launch plumbing (programmatic dependent launch), status
-// codes and the device layouts of the packed weights.
+// Shared pieces of libb200q: launch plumbing (programmatic dependent launch), status codes and the device layouts of
+// the packed weights.
 #pragma once
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
@@ -8,14 +8,6 @@
 #include <cstddef>
 
 #include "../../include/b200q.h"
-
-// The ggml tables are taken from the reference's own table file by path at build time (B200Q_IQ2_TABLES), never
-// re-typed: kmask_iq2xs[8], ksigns_iq2xs[128], ksigns64[128], iq2xxs_grid[256] (engine/iq2_tables.inc:1-117).
-#define GGML_TABLE_BEGIN(type, name, size) static __device__ const type name[size] = {
-#define GGML_TABLE_END() };
-#include B200Q_IQ2_TABLES
-#undef GGML_TABLE_BEGIN
-#undef GGML_TABLE_END
 
 namespace b200q {
 

@@ -32,6 +32,7 @@
 // re-encodes ggml's sign word (four 7-bit fields, s4 in bits 28-31) as four bytes, byte g = field g | bit g of s4 << 7;
 // the spare top bit selects the table's second, identical half of sign words.
 #include "iq2.cuh"
+#include "iq2_tables.cuh"
 #include "moe.cuh"
 
 #include <atomic>
@@ -1098,9 +1099,15 @@ bool iq2_shape_ok(int64_t n, int k) { return n > 0 && n % kIq2Tile == 0 && n <= 
 // the GEMVs stream weights, int8 rows and scales with bulk copies, which need 16-byte aligned addresses
 static bool a16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-int tc_error_read(int clear);   // tc_gemm.cu
-int nv4_error_read(int clear);  // nv4_gemm.cu
-int gemv_error_read(int clear); // gemv_tc.cu
+int iq2_error_read(int clear) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_iq2_error, sizeof(int)) != cudaSuccess) return -1;
+    if (clear) {
+        const int z = 0;
+        cudaMemcpyToSymbol(g_iq2_error, &z, sizeof(int));
+    }
+    return v;
+}
 
 }  // namespace b200q
 
@@ -1143,18 +1150,6 @@ extern "C" int b200q_x_trace(unsigned long long* out) {
     return (int)cudaMemcpyFromSymbol(out, g_x_trace, sizeof(g_x_trace));
 }
 #endif
-
-int b200q_device_error(int clear) {
-    int v = 0;
-    if (cudaMemcpyFromSymbol(&v, g_iq2_error, sizeof(int)) != cudaSuccess) return -1;
-    if (clear) {
-        const int z = 0;
-        cudaMemcpyToSymbol(g_iq2_error, &z, sizeof(int));
-    }
-    const int t = b200q::tc_error_read(clear), f = b200q::nv4_error_read(clear), d = b200q::gemv_error_read(clear);
-    if (t < 0 || f < 0 || d < 0) return -1;
-    return v | (t << 4) | (f << 8) | (d << 12);
-}
 
 int b200q_iq2_gemv(const void* w, int n, int k, const int8_t* xq, const float* xs, int T, float* y, int ldy, int epi,
                    void* stream) {

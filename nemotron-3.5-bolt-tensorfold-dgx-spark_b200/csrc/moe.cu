@@ -7,22 +7,6 @@
 
 namespace b200q {
 
-
-
-// ---------------------------------------------------------------------------------------------------------
-// status plumbing
-// ---------------------------------------------------------------------------------------------------------
-static thread_local int g_last_cuda = 0;
-int status_from(cudaError_t e) {
-    if (e == cudaSuccess) return B200Q_OK;
-    g_last_cuda = (int)e;
-    return B200Q_ECUDA;
-}
-bool pdl_enabled() {
-    static const bool on = [] { const char* e = getenv("B200Q_PDL"); return !(e && atoi(e) == 0); }();
-    return on;
-}
-
 __global__ void quant_rows_k(const void* __restrict__ x, int dtype, int ldx, int8_t* __restrict__ q, int ldq,
                              float* __restrict__ s, int lds, int rows, int k) {
     pdl_wait();
@@ -299,18 +283,6 @@ static ExpertsWs experts_ws(char* base, int R, int H, int F, int n_local) {
 using namespace b200q;
 
 extern "C" {
-
-int b200q_abi(void) { return B200Q_ABI; }
-int b200q_last_cuda_error(void) { return g_last_cuda; }
-const char* b200q_strerror(int status) {
-    switch (status) {
-        case B200Q_OK: return "ok";
-        case B200Q_EINVAL: return "invalid argument (null pointer, shape or alignment)";
-        case B200Q_ENOSPACE: return "workspace or capacity too small";
-        case B200Q_ECUDA: return "CUDA launch error (see b200q_last_cuda_error)";
-        default: return "unknown status";
-    }
-}
 
 int b200q_quant_rows(const void* x, int x_dtype, int ldx, int8_t* q, int ldq, float* s, int lds, int rows, int k,
                      void* stream) {

@@ -39,6 +39,7 @@
 //   X      activations rounded to fp16 once; the MoE's intermediate act = fp16(relu(v)^2).
 // Every barrier wait is bounded (%globaltimer); on a timeout the kernel records an error (b200q_device_error bit 4),
 // waits for its own copies and MMAs, frees its TMEM and returns.  Every copy has one destination, its own CTA.
+#include "iq2_tables.cuh"
 #include "tcgen05.cuh"
 
 namespace b200q {
