@@ -54,7 +54,8 @@ int b200q_last_cuda_error(void);
 const char* b200q_strerror(int status);
 /* Errors the kernels recorded on the current device (a bitmask, 0 if none; bit 0: a streaming GEMV's bounded wait for
  * its copies ran out, so its outputs are incomplete; bit 4: the same in an fp16 tensor-core GEMM; bit 8: in the NVFP4
- * tensor-core GEMM; bit 12: in the Q8_0 decode GEMV); synchronous.  clear != 0 resets it.  No counterpart in libbolt,
+ * tensor-core GEMM; bit 12: in the Q8_0 decode GEMV; bit 16: b200q_kv_append met a position outside its page table or
+ * a table entry outside the cache); synchronous.  clear != 0 resets it.  No counterpart in libbolt,
  * whose kernels do not wait on barriers. */
 int b200q_device_error(int clear);
 
@@ -320,6 +321,36 @@ size_t b200q_moe_decode_noalloc_max_bytes(void);
 int b200q_moe_decode_noalloc(const void* x, const void* logits, const void* up, const void* down, const void* shared_up,
                              const void* shared_down, int T, int H, int F, int E, int topk, int route, const float* bias,
                              float scale, void* out, int out_dtype, int* ridx_out, float* rw_out, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Paged attention of the GQA layers: what stands between the q/k/v projection and o_proj.
+ *
+ * The cache: k_pages and v_pages [pages][hkv][page][d] bf16, the hkv * page * d values of a page contiguous, pages
+ * k_stride / v_stride elements apart (a multiple of 8, so k and v may interleave in one pool).  page: a power of two,
+ * 16 .. 256; d: 64 or 128.
+ * The step: a ragged batch of rows.  Sequence b has rows cu[b] .. cu[b + 1] - 1 and lens[b] cached tokens, the step's
+ * own included, so its row i of r stands at position lens[b] - r + i; the token at position p lives in page
+ * table[b * ldt + p / page], row p % page.  cu [batch + 1], lens [batch] and table [batch][ldt >= width] are int32 on the
+ * device, read by the kernels alone: a captured graph follows their contents.  Rows outside cu[0] .. cu[batch] - 1
+ * (padding) are neither read nor written, nor are rows at a negative position.  batch <= 4096,
+ * width * page <= 2^30.
+ * --------------------------------------------------------------------------------------------------------- */
+
+/* Append (the role of kv_store_k, bolt_kernels.cu:1735, with the steps before it): for each of `rows` rows
+ *   q_out = bf16(rotate(norm(q))),  k_pages[slot] = bf16(rotate(norm(k))),  v_pages[slot] = bf16(v)
+ * q [rows][hq][d], k and v [rows][hkv][d], fp32 or bf16 (x_dtype), rows ldq / ldk / ldv elements apart (16-byte
+ * multiples; the fused projection's output can be passed as it is), q_out [rows][hq][d] bf16, rows ldo apart; q_out may
+ * be q itself.  hq = 0 with q and q_out NULL appends keys and values alone.
+ * norm: x * rsqrt(mean(x^2) + eps) * w over each head, w = q_norm / k_norm [d] (norm_dtype fp32 or bf16), NULL: none.
+ * rotate: the first `rope` values of a head (a multiple of 16, 0: none) in pairs (i, i + rope / 2), or (2i, 2i + 1) when
+ * interleaved, by the angle position * inv_freq[i] (fp32 [rope / 2]).
+ * A row whose position has no table entry, or whose entry is no page of the cache, gets q_out but stores nothing, and sets
+ * bit 16 of b200q_device_error.  Two rows of a call must not name the same slot.  Pointers 16-byte aligned. */
+int b200q_kv_append(const void* q, const void* k, const void* v, int x_dtype, int64_t ldq, int64_t ldk, int64_t ldv,
+                    int rows, int hq, int hkv, int d, void* k_pages, void* v_pages, int64_t k_stride, int64_t v_stride,
+                    int pages, int page, const int* table, int64_t ldt, int width, const int* lens, const int* cu,
+                    int batch, const float* inv_freq, int rope, int interleaved, const void* q_norm, const void* k_norm,
+                    int norm_dtype, float eps, void* q_out, int64_t ldo, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------
  * Synthetic inputs (BASELINE's generators), host and device producing the same bytes.

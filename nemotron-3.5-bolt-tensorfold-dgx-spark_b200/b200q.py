@@ -7,6 +7,7 @@ and calling the sm_100a kernels through ctypes.  Errors raise B200QError with li
 returns void and logs; its C ABI returns -1/-3).  There is no CPU fallback: without libb200q.so, or without a GPU,
 every operator raises.
 """
+import contextlib
 import ctypes
 import json
 import os
@@ -94,6 +95,8 @@ def lib():
             "b200q_quant_nv4_rows": (i32, [vp, i32, i32, i32, i32, vp, vp]),
             "b200q_nv4_gemm_workspace_bytes": (sz, [i32, i32, i32]),
             "b200q_nv4_gemm": (i32, [vp, i32, i32, f32, vp, i32, vp, i32, vp, sz, vp]),
+            "b200q_kv_append": (i32, [vp, vp, vp, i32, i64, i64, i64, i32, i32, i32, i32, vp, vp, i64, i64, i32, i32, vp, i64,
+                                      i32, vp, vp, i32, vp, i32, i32, vp, vp, i32, f32, vp, i64, vp]),
             "b200q_ckpt_open": (vp, [ctypes.c_char_p]),
             "b200q_ckpt_close": (None, [vp]),
             "b200q_ckpt_count": (i64, [vp]),
@@ -553,6 +556,112 @@ def moe_prompt(up, down, E, H, F, counts, offsets, order, topk, x, mo=None, act=
                                   _dtype_code(x), _p(mo), _dtype_code(mo), _p(act) if act is not None else None, ws, wb,
                                   _s()), "moe_prompt")
     return mo
+
+
+# -------------------------------------------------------------------------------------------------------------
+# paged attention (kv_store and the attention between the q/k/v projection and o_proj)
+# -------------------------------------------------------------------------------------------------------------
+def _heads(t, name, device, dtype=None):
+    """rows of heads [rows][heads][d] on `device`, a row's heads contiguous, rows at any pitch -> its pitch"""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise B200QError(EINVAL, f"{name} must be a CUDA tensor")
+    if t.device != device:
+        raise B200QError(EINVAL, f"{name} is on {t.device}, the cache on {device}")
+    if dtype is not None and t.dtype != dtype:
+        raise B200QError(EINVAL, f"{name} must be {dtype}")
+    if t.dim() != 3:
+        raise B200QError(EINVAL, f"{name} must be [rows][heads][d]")
+    n, h, d = t.shape
+    s0, s1, s2 = t.stride()
+    if n * h * d and ((s2 != 1 and d > 1) or (s1 != d and h > 1)):
+        raise B200QError(EINVAL, f"{name}'s heads must be contiguous in a row")
+    return s0 if n > 1 else h * d
+
+
+def _paged(k_pages, v_pages, table, lens, cu):
+    """the cache and the step's description, checked -> the C ABI's arguments
+    (k_pages, v_pages, k_stride, v_stride, pages, page), (table, ldt, width, lens, cu, batch)"""
+    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages"), (table, "table"), (lens, "lens"), (cu, "cu")):
+        if not (isinstance(t, torch.Tensor) and t.is_cuda):
+            raise B200QError(EINVAL, f"{name} must be a CUDA tensor")
+        if t.device != k_pages.device:
+            raise B200QError(EINVAL, f"{name} is on {t.device}, the cache on {k_pages.device}")
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != torch.bfloat16 or \
+            v_pages.dtype != torch.bfloat16:
+        raise B200QError(EINVAL, "k_pages and v_pages must be bf16 [pages][heads][page][d] of one shape")
+    pages, h, page, d = k_pages.shape
+    inner = (page * d, d, 1)
+    if pages * h * page * d == 0 or k_pages.stride()[1:] != inner or v_pages.stride()[1:] != inner:
+        raise B200QError(EINVAL, "a page of the cache must be contiguous and not empty")
+    if table.dim() != 2 or table.dtype != torch.int32 or lens.dim() != 1 or lens.dtype != torch.int32 or cu.dim() != 1 or \
+            cu.dtype != torch.int32:
+        raise B200QError(EINVAL, "table [batch][pages], lens [batch] and cu [batch + 1] must be int32")
+    batch, width = table.shape
+    if batch == 0 or width == 0 or table.stride(1) != 1 or lens.shape[0] != batch or cu.shape[0] != batch + 1 or \
+            lens.stride(0) != 1 or cu.stride(0) != 1:
+        raise B200QError(EINVAL, "table [batch][pages], lens [batch] and cu [batch + 1] must be contiguous and agree")
+    one = h * page * d
+    return ((k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0) if pages > 1 else one,
+             v_pages.stride(0) if pages > 1 else one, pages, page),
+            (table.data_ptr(), table.stride(0) if batch > 1 else width, width, lens.data_ptr(), cu.data_ptr(), batch))
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """a context in which `device` is the current one"""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def k_kv_append(q, k, v, k_pages, v_pages, table, lens, cu, inv_freq=None, interleaved=False, q_norm=None, k_norm=None,
+                eps=1e-6, q_out=None):
+    """A step's keys and values into the paged cache (kv_store), norm and rotation on the way; see b200q_kv_append.
+
+    q [rows][hq][d] (or None), k and v [rows][hkv][d]: fp32 or bf16, rows at any 16-byte pitch (views of the fused
+    projection's output); k_pages / v_pages [pages][hkv][page][d] bf16; table [batch][width], lens [batch],
+    cu [batch + 1] int32; inv_freq: fp32 [rope / 2], rotates the first `rope` values of each query and key head;
+    q_norm / k_norm [d]: weights of the RMS norm of each head.  -> q_out [rows][hq][d] bf16 (padding rows unwritten)"""
+    cache, seqs = _paged(k_pages, v_pages, table, lens, cu)
+    dev = k_pages.device
+    ldk, ldv = _heads(k, "k", dev), _heads(v, "v", dev, k.dtype)
+    hkv, d = k_pages.shape[1], k_pages.shape[3]
+    if k.shape != v.shape or k.shape[1:] != (hkv, d):
+        raise B200QError(EINVAL, f"k and v must be [rows][{hkv}][{d}] like the cache")
+    rows, hq, ldq, ldo, qp, op = k.shape[0], 0, 0, 0, None, None
+    if q is not None:
+        ldq = _heads(q, "q", dev, k.dtype)
+        if q.shape[0] != rows or q.shape[2] != d:
+            raise B200QError(EINVAL, f"q must be [{rows}][heads][{d}]")
+        hq = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty(rows, hq, d, dtype=torch.bfloat16, device=dev)
+        ldo = _heads(q_out, "q_out", dev, torch.bfloat16)
+        if q_out.shape != q.shape:
+            raise B200QError(EINVAL, "q_out must have q's shape")
+        qp, op = q.data_ptr(), q_out.data_ptr()
+    rope = 0
+    if inv_freq is not None:
+        if not (isinstance(inv_freq, torch.Tensor) and inv_freq.device == dev and inv_freq.dtype == torch.float32 and
+                inv_freq.dim() == 1 and inv_freq.is_contiguous()):
+            raise B200QError(EINVAL, "inv_freq must be a contiguous fp32 CUDA tensor beside the cache")
+        rope = 2 * inv_freq.numel()
+    norm_dtype = F32
+    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if w is None:
+            continue
+        if not (isinstance(w, torch.Tensor) and w.device == dev and w.shape == (d,) and w.is_contiguous()):
+            raise B200QError(EINVAL, f"{name} must be a contiguous [{d}] CUDA tensor beside the cache")
+        norm_dtype = _dtype_code(w)
+    if q_norm is not None and k_norm is not None and q_norm.dtype != k_norm.dtype:
+        raise B200QError(EINVAL, "q_norm and k_norm must have one dtype")
+    if rows == 0:
+        return q_out
+    with _on(dev):
+        _check(lib().b200q_kv_append(qp, k.data_ptr(), v.data_ptr(), _dtype_code(k), ldq, ldk, ldv, rows, hq, hkv, d,
+                                     *cache, *seqs, inv_freq.data_ptr() if rope else None, rope, 1 if interleaved else 0,
+                                     _p(q_norm), _p(k_norm), norm_dtype, float(eps), op, ldo, _s()), "k_kv_append")
+    return q_out
 
 
 # -------------------------------------------------------------------------------------------------------------
