@@ -55,7 +55,9 @@ const char* b200q_strerror(int status);
 /* Errors the kernels recorded on the current device (a bitmask, 0 if none; bit 0: a streaming GEMV's bounded wait for
  * its copies ran out, so its outputs are incomplete; bit 4: the same in an fp16 tensor-core GEMM; bit 8: in the NVFP4
  * tensor-core GEMM; bit 12: in the Q8_0 decode GEMV; bit 16: b200q_kv_append met a position outside its page table or
- * a table entry outside the cache); synchronous.  clear != 0 resets it.  No counterpart in libbolt,
+ * a table entry outside the cache; bit 20: a bounded wait of the paged attention ran out, bit 21: it met a table entry
+ * outside the cache or a length outside 0 .. width * page, bit 22: a sequence had more rows than max_rows);
+ * synchronous.  clear != 0 resets it.  No counterpart in libbolt,
  * whose kernels do not wait on barriers. */
 int b200q_device_error(int clear);
 
@@ -351,6 +353,31 @@ int b200q_kv_append(const void* q, const void* k, const void* v, int x_dtype, in
                     int pages, int page, const int* table, int64_t ldt, int width, const int* lens, const int* cu,
                     int batch, const float* inv_freq, int rope, int interleaved, const void* q_norm, const void* k_norm,
                     int norm_dtype, float eps, void* q_out, int64_t ldo, void* stream);
+
+/* Attention over the cache (the roles of attn_part_k / attn_blk_part_k, bolt_kernels.cu:1779-2009, and attn_mma_part_k /
+ * attn_mma2_part_k, bolt_mma.cu:1406-1724, with their combines): for each row of the step and query head h
+ *   out = sum_j p_j v_j / sum_j p_j,   p_j = exp(s_j),   s_j = scale q . k_j, or softcap tanh(scale q . k_j / softcap)
+ * over the keys j of kv head h / (hq / hkv) with position - window < j <= position (window 0: all up to the position).
+ * A row that sees no key gets zeros.  q [rows][hq][d] and out [rows][hq][d] bf16, rows ldq / ldo elements apart (multiples
+ * of 8), 16-byte aligned, not overlapping.  Scores, sums and accumulators are fp32; the probabilities are rounded to bf16
+ * for the product with v.  scale > 0, softcap >= 0 (0: none).
+ * decode: up to 16 rows a sequence (one new token, or a verify window).  prompt: any number.  max_rows >= the rows of
+ * every sequence (a sequence with more sets bit 22 of b200q_device_error, and some of its rows are left out).
+ * A table entry outside the cache reads as zeros, a length outside 0 .. width * page is brought inside; both set bit 21.
+ * workspace: >= the *_workspace_bytes query, 16-byte aligned, contents of no matter before and after a call; two calls
+ * that may overlap need one each. */
+size_t b200q_attn_decode_workspace_bytes(int hq, int hkv, int d, int max_rows);
+int b200q_attn_decode(const void* q, int64_t ldq, int rows, int hq, const void* k_pages, const void* v_pages,
+                      int64_t k_stride, int64_t v_stride, int pages, int page, int hkv, int d, const int* table,
+                      int64_t ldt, int width, const int* lens, const int* cu, int batch, int max_rows, float scale,
+                      float softcap, int window, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
+                      void* stream);
+size_t b200q_attn_prompt_workspace_bytes(int hq, int hkv, int d, int rows, int max_rows, int batch);
+int b200q_attn_prompt(const void* q, int64_t ldq, int rows, int hq, const void* k_pages, const void* v_pages,
+                      int64_t k_stride, int64_t v_stride, int pages, int page, int hkv, int d, const int* table,
+                      int64_t ldt, int width, const int* lens, const int* cu, int batch, int max_rows, float scale,
+                      float softcap, int window, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
+                      void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------
  * Synthetic inputs (BASELINE's generators), host and device producing the same bytes.

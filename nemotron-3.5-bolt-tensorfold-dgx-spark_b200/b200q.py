@@ -97,6 +97,12 @@ def lib():
             "b200q_nv4_gemm": (i32, [vp, i32, i32, f32, vp, i32, vp, i32, vp, sz, vp]),
             "b200q_kv_append": (i32, [vp, vp, vp, i32, i64, i64, i64, i32, i32, i32, i32, vp, vp, i64, i64, i32, i32, vp, i64,
                                       i32, vp, vp, i32, vp, i32, i32, vp, vp, i32, f32, vp, i64, vp]),
+            "b200q_attn_decode_workspace_bytes": (sz, [i32, i32, i32, i32]),
+            "b200q_attn_decode": (i32, [vp, i64, i32, i32, vp, vp, i64, i64, i32, i32, i32, i32, vp, i64, i32, vp, vp, i32,
+                                        i32, f32, f32, i32, vp, i64, vp, sz, vp]),
+            "b200q_attn_prompt_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
+            "b200q_attn_prompt": (i32, [vp, i64, i32, i32, vp, vp, i64, i64, i32, i32, i32, i32, vp, i64, i32, vp, vp, i32,
+                                        i32, f32, f32, i32, vp, i64, vp, sz, vp]),
             "b200q_ckpt_open": (vp, [ctypes.c_char_p]),
             "b200q_ckpt_close": (None, [vp]),
             "b200q_ckpt_count": (i64, [vp]),
@@ -662,6 +668,51 @@ def k_kv_append(q, k, v, k_pages, v_pages, table, lens, cu, inv_freq=None, inter
                                      *cache, *seqs, inv_freq.data_ptr() if rope else None, rope, 1 if interleaved else 0,
                                      _p(q_norm), _p(k_norm), norm_dtype, float(eps), op, ldo, _s()), "k_kv_append")
     return q_out
+
+
+def _attend(what, q, k_pages, v_pages, table, lens, cu, max_rows, scale, softcap, window, out):
+    cache, seqs = _paged(k_pages, v_pages, table, lens, cu)
+    dev = k_pages.device
+    hkv, d = k_pages.shape[1], k_pages.shape[3]
+    ldq = _heads(q, "q", dev, torch.bfloat16)
+    rows, hq = q.shape[:2]
+    if q.shape[2] != d or hq % hkv:
+        raise B200QError(EINVAL, f"q must be [rows][a multiple of {hkv}][{d}]")
+    if out is None:
+        out = torch.empty(rows, hq, d, dtype=torch.bfloat16, device=dev)
+    elif out.shape != q.shape:
+        raise B200QError(EINVAL, "out must have q's shape")
+    ldo = _heads(out, "out", dev, torch.bfloat16)
+    if rows == 0:
+        return out
+    L = lib()
+    with _on(dev):
+        # scratch of this call alone: calls on other streams, and captured ones, have their own
+        if what == "attn_decode":
+            ws = torch.empty(L.b200q_attn_decode_workspace_bytes(hq, hkv, d, max_rows), dtype=torch.uint8, device=dev)
+            fn = L.b200q_attn_decode
+        else:
+            ws = torch.empty(L.b200q_attn_prompt_workspace_bytes(hq, hkv, d, rows, max_rows, seqs[5]), dtype=torch.uint8,
+                             device=dev)
+            fn = L.b200q_attn_prompt
+        _check(fn(q.data_ptr(), ldq, rows, hq, *cache, hkv, d, *seqs, max_rows, d ** -0.5 if scale is None else scale, softcap,
+                  window, out.data_ptr(), ldo, ws.data_ptr(), ws.numel(), _s()), what)
+    return out
+
+
+def attn_decode(q, k_pages, v_pages, table, lens, cu, max_rows, scale=None, softcap=0.0, window=0, out=None):
+    """Attention of a decode or verify step (up to 16 rows a sequence) over the paged cache; see b200q_attn_decode.
+
+    q [rows][hq][d] bf16 (k_kv_append's q_out); the cache and the step as k_kv_append takes them; max_rows: the most rows of
+    a sequence; scale: 1 / sqrt(d) by default; softcap: scores capped by its tanh (0: not); window: keys a row sees at most,
+    its own included (0: all before it).  -> out [rows][hq][d] bf16 (padding rows unwritten)"""
+    return _attend("attn_decode", q, k_pages, v_pages, table, lens, cu, max_rows, scale, softcap, window, out)
+
+
+def attn_prompt(q, k_pages, v_pages, table, lens, cu, max_rows, scale=None, softcap=0.0, window=0, out=None):
+    """Attention of prompt chunks (any number of rows a sequence) over the paged cache, which holds what came before the
+    chunk and the chunk's own keys and values; arguments as attn_decode's"""
+    return _attend("attn_prompt", q, k_pages, v_pages, table, lens, cu, max_rows, scale, softcap, window, out)
 
 
 # -------------------------------------------------------------------------------------------------------------

@@ -1,0 +1,654 @@
+// Attention of a step's few rows over a paged key/value cache (the role of attn_part_k / attn_blk_part_k and their
+// combine, bolt_kernels.cu:1779-2009): per row  o = sum_j p_j v_j / sum_j p_j,  p_j = exp(cap(scale q . k_j) - m)  over the
+// keys it sees, in one pass over the cache with the running maximum m and sum.
+//
+// Bound by HBM: every key and value a row sees is read once for all rows and query heads of its kv head.
+//
+// Work.  A row block is up to 8 NT rows (row = token * group + query head of the group) of one (sequence, kv head); its
+// keys are cut into units of 16 (within one page, since pages hold 16 or more).  The units of all row blocks stand in one
+// line, and each CTA takes an equal share of the line: ragged lengths and few long sequences load every SM alike, whatever
+// the lengths on the device are.  A row block cut by a share's end leaves partial sums (fp32), which a second small kernel
+// joins in the line's order, so results do not depend on timing.
+//
+// A CTA is one producer warp, which walks the share and fills a ring of units by TMA (128-byte swizzle), and eight
+// consumer warps, which take the ring's units in turn.  Scores are formed transposed, S^T = K Q^T: 16 keys are the rows of
+// an m16n8k16 and 8 query rows its columns, so a group of 4 or 8 query heads wastes half or none of it (16 x 8 the
+// other way round would waste three quarters).  The probabilities' accumulator becomes the B operand of O^T += V^T P^T by one
+// 8 x 8 transpose (movmatrix) each; P is rounded to bf16 there, V's type: 2^-9 relative on weights that are summed with
+// independent signs, below the output's own rounding.  m, the sum and O stay in fp32.
+#include "attn.cuh"
+#include "tcgen05.cuh"
+
+#include <climits>
+
+namespace b200q {
+
+__device__ int g_attn_error;   // bit 0: a wait ran out, bit 1: a page table or length out of range, bit 2: over max_rows
+
+int attn_error_read(int clear) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_attn_error, sizeof(int)) != cudaSuccess) return -1;
+    if (clear) {
+        const int z = 0;
+        cudaMemcpyToSymbol(g_attn_error, &z, sizeof(int));
+    }
+    return v;
+}
+
+int attn_sms() {
+    static int sms[64] = {0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) dev = 0;
+    if (!sms[dev]) {
+        int v = 0;
+        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
+        sms[dev] = v > 0 ? v : 148;
+    }
+    return sms[dev];
+}
+
+bool kv_tensor_map(CUtensorMap* m, const void* base, int64_t page_stride, int pages, int page, int heads, int d, int box_rows) {
+    typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static Encode encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return (Encode)f;
+    }();
+    if (!encode) return false;
+    const cuuint64_t dims[5] = {64, (cuuint64_t)page, (cuuint64_t)d / 64, (cuuint64_t)heads, (cuuint64_t)pages};
+    const cuuint64_t strides[4] = {(cuuint64_t)d * 2, 128, (cuuint64_t)page * d * 2, (cuuint64_t)page_stride * 2};
+    const cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)d / 64, 1, 1}, one[5] = {1, 1, 1, 1, 1};
+    return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, one,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+namespace {
+
+constexpr int kWarps = 8;                    // consumer warps
+constexpr int kUnit = 16;                    // keys a unit
+constexpr int kRing = 128 * 1024;            // bytes of units in flight
+constexpr int kMaxCtas = 160;                // shares the workspace holds
+constexpr int kJoin = 8;                     // accumulator fragments a join pass moves per warp (32 KB in all)
+constexpr int kMinUnits = 8;                 // a share is not smaller: one unit a warp
+
+template <int D, int NT>
+struct Shape {
+    static constexpr int kRows = 8 * NT;                     // rows of a row block
+    static constexpr int kBytes = kUnit * D * 4;             // a unit: K [D / 64][16][128 B], then V
+    static constexpr int kStages = kRing / kBytes;           // a multiple of kWarps: a warp meets its own stages only
+    static constexpr int kFrags = D / 16 * NT;               // accumulator fragments (16 x 8) of a warp
+    static constexpr size_t kQ = (size_t)kRows * D * 2;
+    static constexpr size_t kSlot = (size_t)kRows * (D + 2); // floats of a partial: O [rows][D], m [rows], sum [rows]
+    static size_t smem(int batch) {
+        return 1024 + kRing + kQ + (size_t)kWarps * kJoin * 512 + (size_t)kWarps * kRows * 8 + kStages * 16 +
+               (size_t)kRows * 8 + (size_t)(batch + 1) * 8;
+    }
+};
+
+struct Desc {   // what a share left to join: n partials of rows row0 .. of a sequence starting at row cu0, kv head h
+    int n, cu0, row0, nrows, h, pad[3];
+};
+
+// a row block's keys: units u0 .. u0 + n - 1 hold every key that one of its rows sees
+struct Span {
+    int u0, n, lo, hi, p0, p1;   // keys lo .. hi - 1; positions of its first and last row
+};
+template <int ROWS>
+__device__ __forceinline__ bool row_block(int r, int len, int rb, int group, int window, Span& s) {
+    const int first = rb * ROWS, all = r * group;
+    if (first >= all) return false;
+    const int last = min(first + ROWS, all) - 1;
+    s.p0 = len - r + first / group;
+    s.p1 = len - r + last / group;
+    s.hi = max(s.p1 + 1, 0);
+    s.lo = min(max(0, s.p0 - window + 1), s.hi);
+    s.u0 = s.lo / kUnit;
+    s.n = s.hi > s.lo ? (s.hi + kUnit - 1) / kUnit - s.u0 : 0;
+    return true;
+}
+
+__device__ __forceinline__ void seq_sizes(const AttnArgs& a, int b, int& cu0, int& r, int& len) {
+    cu0 = min(max(a.s.cu[b], 0), a.rows);
+    r = min(max(a.s.cu[b + 1], cu0), a.rows) - cu0;
+    len = min(max(a.s.lens[b], 0), a.s.width << a.page_log2);
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *(uint32_t*)&v;
+}
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// the line of units: pre[b] counts those of the sequences before b
+struct Line {
+    const long long* pre;
+    int batch;
+};
+// One CTA's next piece: a row block (b, h, rb) and its units from .. to - 1 (counted from the block's first), cut by the
+// share's end.  at: the line's position of the piece, advanced past it.
+struct Piece {
+    int b, h, rb, cu0, r, len;
+    Span s;
+    long long begin, end;    // the row block on the line
+    long long from, to;      // the piece on the line
+};
+template <int ROWS>
+__device__ __forceinline__ void next_piece(const AttnArgs& a, const Line& l, int nrb, long long at, long long stop, Piece& p) {
+    int lo = 0, hi = l.batch - 1;   // the last b with pre[b] <= at: sequences without units are skipped
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (l.pre[mid] <= at) lo = mid; else hi = mid - 1;
+    }
+    p.b = lo;
+    seq_sizes(a, lo, p.cu0, p.r, p.len);
+    const long long a_head = (l.pre[lo + 1] - l.pre[lo]) / a.hkv;
+    long long rest = at - l.pre[lo];
+    p.h = (int)(rest / a_head);
+    rest -= p.h * a_head;
+    long long before = 0;
+    for (p.rb = 0; p.rb < nrb; p.rb++) {
+        if (!row_block<ROWS>(p.r, p.len, p.rb, a.group, a.window, p.s)) break;
+        const int c = max(p.s.n, 1);
+        if (rest < before + c) {
+            p.begin = l.pre[lo] + p.h * a_head + before;
+            p.end = p.begin + c;
+            break;
+        }
+        before += c;
+    }
+    p.from = at;
+    p.to = min(stop, p.end);
+}
+
+__device__ __forceinline__ long long share_start(long long total, int k, int shares) { return total * k / shares; }
+
+template <int D, int NT>
+__global__ void __launch_bounds__((kWarps + 1) * 32, 1)
+attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, AttnArgs a) {
+    using S = Shape<D, NT>;
+    constexpr int RB = S::kRows, NS = S::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw), ring = (raw + 1023) & ~1023u;
+    uint8_t* base = smem_raw + (ring - raw);
+    uint2* qs = (uint2*)(base + kRing);                                   // Q fragments [D / 16][NT][32]
+    float4* jo = (float4*)(base + kRing + S::kQ);                         // join: [kWarps][kJoin][32]
+    float* jm = (float*)(base + kRing + S::kQ + kWarps * kJoin * 512);    // join: m [kWarps][RB], then sums
+    float* jl = jm + kWarps * RB;
+    float* jt = jl + kWarps * RB;                                          // joined m [RB], sum [RB]
+    const uint32_t full = ring + kRing + (uint32_t)S::kQ + kWarps * kJoin * 512 + (kWarps + 1) * RB * 8, empty = full + NS * 8;
+    long long* pre = (long long*)(base + (empty + NS * 8 - ring));
+    __shared__ long long warp_sum[kWarps + 1];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < NS; i++) { tc_mbar_init(full + i * 8, 1); tc_mbar_init(empty + i * 8, 1); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tma_prefetch(&mk);
+        tma_prefetch(&mv);
+    }
+    pdl_wait();
+    pdl_trigger();
+
+    // the line: an exclusive sum of the sequences' units, 288 sequences at a time
+    const int nrb = (a.max_rows * a.group + RB - 1) / RB;
+    long long carry = 0;
+    if (tid == 0) pre[0] = 0;
+    for (int b0 = 0; b0 < a.s.batch; b0 += (kWarps + 1) * 32) {
+        const int b = b0 + tid;
+        long long c = 0;
+        if (b < a.s.batch) {
+            int cu0, r, len;
+            Span s;
+            seq_sizes(a, b, cu0, r, len);
+            for (int rb = 0; rb < nrb && row_block<RB>(r, len, rb, a.group, a.window, s); rb++) c += max(s.n, 1);
+            c *= a.hkv;
+            if (blockIdx.x == 0 && (r > a.max_rows || len != a.s.lens[b])) atomicOr(&g_attn_error, r > a.max_rows ? 4 : 2);
+        }
+        long long sum = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(~0u, sum, o);
+            if (lane >= o) sum += v;
+        }
+        if (lane == 31) warp_sum[warp] = sum;
+        __syncthreads();
+        long long below = carry;
+        for (int w = 0; w <= kWarps; w++) {
+            if (w < warp) below += warp_sum[w];
+            carry += warp_sum[w];
+        }
+        if (b < a.s.batch) pre[b + 1] = below + sum;
+        __syncthreads();
+    }
+    const long long total = carry;
+    const int shares = (int)min((long long)gridDim.x, (total + kMinUnits - 1) / kMinUnits);
+    Desc* desc = (Desc*)a.ws;
+    float* slots = (float*)((uint8_t*)a.ws + kMaxCtas * sizeof(Desc));
+    if ((int)blockIdx.x >= shares) {
+        if (tid == 0) desc[blockIdx.x].n = 0;
+        return;
+    }
+    const long long begin = share_start(total, blockIdx.x, shares), end = share_start(total, blockIdx.x + 1, shares);
+    const Line line = {pre, a.s.batch};
+    Piece p;
+    int ordinal = 0;   // units of the share before the piece
+    bool dead = false;
+
+    if (warp == kWarps) {
+        // ---------------------------------------------------------------- producer
+        bool bad_page = false;
+        int issued = 0;
+        for (long long at = begin; at < end; at = p.to) {
+            next_piece<RB>(a, line, nrb, at, end, p);
+            const int n = p.s.n ? (int)(p.to - p.from) : 0, u0 = p.s.u0 + (int)(p.from - p.begin);
+            const int* tab = a.s.table + p.b * a.s.ldt;
+            int next = 0;
+            if (lane < n) next = tab[((u0 + lane) * kUnit) >> a.page_log2];
+            for (int i0 = 0; i0 < n; i0 += 32) {
+                const int mine = next;
+                if (i0 + 32 + lane < n) next = tab[((u0 + i0 + 32 + lane) * kUnit) >> a.page_log2];   // a round ahead
+                for (int i = 0; i < min(32, n - i0); i++) {
+                    int page = __shfl_sync(~0u, mine, i);
+                    if (page < 0 || page >= a.pages) { bad_page = true; page = a.pages; }   // past the end: TMA fills zeros
+                    const int o = ordinal + i0 + i, st = o % NS;
+                    if (lane == 0 && !dead) {
+                        if (!tc_mbar_wait(empty + st * 8, (o / NS & 1) ^ 1)) dead = true;
+                        else {
+                            const uint32_t dst = ring + st * S::kBytes, bar = full + st * 8;
+                            const int row = ((u0 + i0 + i) * kUnit) & ((1 << a.page_log2) - 1);
+                            tc_mbar_arrive_tx(bar, S::kBytes);
+                            tma_kv(dst, &mk, row, p.h, page, bar);
+                            tma_kv(dst + S::kBytes / 2, &mv, row, p.h, page, bar);
+                            issued = o + 1;
+                        }
+                    }
+                }
+            }
+            ordinal += n;
+        }
+        if (lane == 0) {
+            if (dead) atomicOr(&g_attn_error, 1);
+            // the last copies have landed before the block ends, whatever became of their readers
+            for (int o = max(0, issued - NS); o < issued; o++) tc_mbar_wait(full + (o % NS) * 8, o / NS & 1);
+            if (bad_page) atomicOr(&g_attn_error, 2);
+        }
+        return;
+    }
+
+    // ---------------------------------------------------------------- consumers
+    const int g = lane >> 2, t = lane & 3;
+    const uint32_t krow = lane & 15, kchunk = lane >> 4;                              // ldmatrix: keys x 16-byte chunks
+    const uint32_t vrow = (lane & 7) + ((lane >> 4) & 1) * 8, vchunk = (lane >> 3) & 1;
+    const float c = a.c;
+    if (tid == 0) desc[blockIdx.x].n = 0;
+    for (long long at = begin; at < end; at = p.to) {
+        next_piece<RB>(a, line, nrb, at, end, p);
+        const int n = p.s.n ? (int)(p.to - p.from) : 0, u0 = p.s.u0 + (int)(p.from - p.begin);
+        const int row0 = p.rb * RB, rows = min(RB, p.r * a.group - row0);
+        // Q in fragment order: fragment (kk, nt), lane (g, t): values 16 kk + 2 t, + 1 and + 8, + 9 of row 8 nt + g
+        consumers_sync();
+        for (int i = tid; i < D / 16 * NT * 32; i += kWarps * 32) {
+            const int l = i & 31, nt = (i >> 5) % NT, kk = (i >> 5) / NT, row = nt * 8 + (l >> 2);
+            uint2 v = make_uint2(0, 0);
+            if (row < rows) {
+                const int rr = row0 + row, tok = rr / a.group;
+                const uint32_t* src = (const uint32_t*)(a.q + (p.cu0 + tok) * a.ldq + (int64_t)(p.h * a.group + rr - tok * a.group) * D +
+                                                        kk * 16 + (l & 3) * 2);
+                v = make_uint2(src[0], src[4]);
+            }
+            qs[i] = v;
+        }
+        consumers_sync();
+        uint2 qr[NT <= 2 ? D / 16 * NT : 1];
+        if (NT <= 2) {
+#pragma unroll
+            for (int i = 0; i < D / 16 * NT; i++) qr[i < (NT <= 2 ? D / 16 * NT : 1) ? i : 0] = qs[i * 32 + lane];
+        }
+        int place[NT][2];   // positions of this lane's columns (rows 8 nt + 2 t, + 1); none: before every key
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int row = nt * 8 + t * 2 + j;
+                place[nt][j] = row < rows ? p.len - p.r + (row0 + row) / a.group : -1;
+            }
+        float m[NT][2], sum[NT][2], o[D / 16][NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            sum[nt][0] = sum[nt][1] = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < D / 16; mt++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[mt][nt][j] = 0.f;
+        }
+        // the warp's units: ordinals congruent to it
+        for (int i = (warp - ordinal) & (kWarps - 1); i < n; i += kWarps) {
+            const int od = ordinal + i, st = od % NS, key0 = (u0 + i) * kUnit;
+            if (!dead && !tc_mbar_wait(full + st * 8, od / NS & 1)) { dead = true; if (lane == 0) atomicOr(&g_attn_error, 1); }
+            dead = __any_sync(~0u, dead);
+            if (dead) continue;
+            const uint32_t kt = ring + st * S::kBytes, vt = kt + S::kBytes / 2;
+            bool fenced = false;
+            if (key0 < p.s.lo || key0 + kUnit > p.s.hi) {
+                // values that no row sees may hold anything, and 0 * NaN is NaN: they become zero
+                for (int j = lane; j < kUnit * D / 8; j += 32) {
+                    const int row = (j / 8) % kUnit, key = key0 + row;
+                    if (key < p.s.lo || key >= p.s.hi) sts128(vt + j * 16, make_uint4(0, 0, 0, 0));
+                }
+                __syncwarp();
+                fenced = true;
+            }
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) s[nt][j] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; kk++) {
+                uint32_t k4[4];
+                const uint32_t ch = 2 * kk + kchunk;
+                ldsm4(k4, kt + (ch >> 3) * (kUnit * 128) + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4));
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    const uint2 b = NT <= 2 ? qr[NT <= 2 ? kk * NT + nt : 0] : qs[(kk * NT + nt) * 32 + lane];
+                    mma(s[nt], k4, b.x, b.y);
+                }
+            }
+            const bool whole = key0 + kUnit - 1 <= p.s.p0 && key0 > p.s.p1 - a.window;   // every row sees every key
+            uint32_t pb[NT][2];
+            bool moved = false;
+            float scale[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                if (a.cap_in != 0.f)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[nt][j] = capped(s[nt][j], a.cap_in);
+                if (!whole)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int key = key0 + g + (j >> 1) * 8, at_ = place[nt][j & 1];
+                        if (key > at_ || key <= at_ - a.window) s[nt][j] = -INFINITY;
+                    }
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    float x = fmaxf(s[nt][j], s[nt][j + 2]);
+                    x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
+                    const float mn = fmaxf(m[nt][j], x * c), mz = mn == -INFINITY ? 0.f : mn;
+                    moved |= mn > m[nt][j];
+                    scale[nt][j] = ex2(m[nt][j] - mz);   // 0 for the first keys
+                    m[nt][j] = mn;
+                    s[nt][j] = ex2(fmaf(s[nt][j], c, -mz));
+                    s[nt][j + 2] = ex2(fmaf(s[nt][j + 2], c, -mz));
+                    sum[nt][j] = sum[nt][j] * scale[nt][j] + (s[nt][j] + s[nt][j + 2]);
+                }
+                pb[nt][0] = transpose8(pack_bf16(s[nt][0], s[nt][1]));
+                pb[nt][1] = transpose8(pack_bf16(s[nt][2], s[nt][3]));
+            }
+            if (__any_sync(~0u, moved)) {
+#pragma unroll
+                for (int mt = 0; mt < D / 16; mt++)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) o[mt][nt][j] *= scale[nt][j & 1];
+            }
+#pragma unroll
+            for (int mt = 0; mt < D / 16; mt++) {
+                uint32_t v4[4];
+                const uint32_t ch = 2 * mt + vchunk;
+                ldsm4t(v4, vt + (ch >> 3) * (kUnit * 128) + vrow * 128 + (((ch & 7) ^ (vrow & 7)) << 4));
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) mma(o[mt][nt], v4, pb[nt][0], pb[nt][1]);
+            }
+            if (fenced) tc_fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) tc_mbar_arrive(empty + st * 8);
+        }
+        ordinal += n;
+
+        // join the warps: m and the sum first, then the accumulators, kJoin fragments a pass
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float x = sum[nt][j];
+                x += __shfl_xor_sync(~0u, x, 4);
+                x += __shfl_xor_sync(~0u, x, 8);
+                x += __shfl_xor_sync(~0u, x, 16);
+                if (g == 0) {
+                    jm[warp * RB + nt * 8 + t * 2 + j] = m[nt][j];
+                    jl[warp * RB + nt * 8 + t * 2 + j] = x;
+                }
+            }
+        consumers_sync();
+        float scale[NT][2];   // this warp's part of the joined scale, for this lane's columns
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int row = nt * 8 + t * 2 + j;
+                float x = -INFINITY, y = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) x = fmaxf(x, jm[w * RB + row]);
+                const float z = x == -INFINITY ? 0.f : x;
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) y += jl[w * RB + row] * ex2(jm[w * RB + row] - z);
+                scale[nt][j] = ex2(m[nt][j] - z);
+                if (tid < 4) { jt[row] = x; jt[RB + row] = y; }
+            }
+        const bool complete = p.from == p.begin && p.to == p.end;
+        float* slot = slots + ((size_t)blockIdx.x * 2 + (p.from == p.begin ? 1 : 0)) * S::kSlot;
+#pragma unroll
+        for (int pass = 0; pass < (S::kFrags + kJoin - 1) / kJoin; pass++) {
+#pragma unroll
+            for (int k = 0; k < kJoin; k++) {
+                const int f = pass * kJoin + k;
+                if (f >= S::kFrags) break;
+                float(&v)[4] = o[f / NT][f % NT];
+                jo[(warp * kJoin + k) * 32 + lane] = make_float4(v[0] * scale[f % NT][0], v[1] * scale[f % NT][1],
+                                                                 v[2] * scale[f % NT][0], v[3] * scale[f % NT][1]);
+            }
+            consumers_sync();
+            const int f = pass * kJoin + warp;
+            if (f < S::kFrags) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) {
+                    const float4 x = jo[(w * kJoin + warp) * 32 + lane];
+                    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+                }
+                const int d0 = f / NT * 16, r0 = f % NT * 8;
+                if (complete) {
+                    const float l0 = jt[RB + r0 + t * 2], l1 = jt[RB + r0 + t * 2 + 1];
+                    const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;   // no key seen: zeros
+                    const uint32_t lo = transpose8(pack_bf16(v.x * i0, v.y * i1)), hi = transpose8(pack_bf16(v.z * i0, v.w * i1));
+                    if (r0 + g < rows) {
+                        const int rr = row0 + r0 + g, tok = rr / a.group;
+                        uint32_t* dst = (uint32_t*)(a.out + (p.cu0 + tok) * a.ldo +
+                                                    (int64_t)(p.h * a.group + rr - tok * a.group) * D + d0 + t * 2);
+                        dst[0] = lo;
+                        dst[4] = hi;
+                    }
+                } else {
+                    float* s0 = slot + (r0 + t * 2) * D + d0 + g;
+                    s0[0] = v.x; s0[D] = v.y; s0[8] = v.z; s0[D + 8] = v.w;
+                }
+            }
+            consumers_sync();
+        }
+        if (!complete) {
+            if (tid < 2 * RB) slot[RB * D + tid] = jt[tid];
+            if (tid == 0 && p.from == p.begin) {
+                const long long last = p.end - 1;
+                int k = (int)(last * shares / total);
+                while (share_start(total, k + 1, shares) <= last) k++;
+                Desc& d = desc[blockIdx.x];
+                d.n = k - blockIdx.x + 1;
+                d.cu0 = p.cu0; d.row0 = row0; d.nrows = rows; d.h = p.h;
+            }
+        }
+    }
+}
+
+// the row blocks that a share's end cut: partial 0 is the share's last, the others the first of the shares after it
+template <int D, int NT>
+__global__ void __launch_bounds__(256) attn_join_k(AttnArgs a) {
+    using S = Shape<D, NT>;
+    constexpr int RB = S::kRows, V = D / 32;
+    __shared__ float weight[8][kMaxCtas];
+    pdl_wait();
+    pdl_trigger();
+    const Desc d = ((const Desc*)a.ws)[blockIdx.x];
+    if (d.n <= 0) return;
+    const float* slots = (const float*)((const uint8_t*)a.ws + kMaxCtas * sizeof(Desc));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto slot = [&](int i) { return slots + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * S::kSlot; };
+    for (int r = warp; r < d.nrows; r += 8) {
+        float top = -INFINITY, sum = 0.f;
+        for (int i = lane; i < d.n; i += 32) top = fmaxf(top, slot(i)[RB * D + r]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+        const float z = top == -INFINITY ? 0.f : top;
+        for (int i = lane; i < d.n; i += 32) {
+            const float w = ex2(slot(i)[RB * D + r] - z);
+            weight[warp][i] = w;
+            sum += w * slot(i)[RB * D + RB + r];
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        __syncwarp();
+        float acc[V] = {};
+#pragma unroll 4
+        for (int i = 0; i < d.n; i++) {
+            const float* p = slot(i) + r * D + lane * V;
+            const float w = weight[warp][i];
+            float x[V];
+            if (V == 4) *(float4*)x = *(const float4*)p; else *(float2*)x = *(const float2*)p;
+#pragma unroll
+            for (int j = 0; j < V; j++) acc[j] = fmaf(w, x[j], acc[j]);
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int rr = d.row0 + r, tok = rr / a.group;
+        uint32_t* dst = (uint32_t*)(a.out + (d.cu0 + tok) * a.ldo + (int64_t)(d.h * a.group + rr - tok * a.group) * D + lane * V);
+#pragma unroll
+        for (int j = 0; j < V / 2; j++) dst[j] = pack_bf16(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+        __syncwarp();
+    }
+}
+
+template <int D, int NT>
+cudaError_t launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& a, cudaStream_t s) {
+    const size_t smem = Shape<D, NT>::smem(a.s.batch);
+    cudaError_t e = cudaFuncSetAttribute(attn_rows_k<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    const int ctas = min(attn_sms(), kMaxCtas);
+    e = launch(attn_rows_k<D, NT>, dim3(ctas), dim3((kWarps + 1) * 32), smem, s, mk, mv, a);
+    if (e != cudaSuccess) return e;
+    return launch(attn_join_k<D, NT>, dim3(ctas), dim3(256), 0, s, a);
+}
+
+int row_tiles(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+
+bool attn_args_ok(const void* q, int64_t ldq, int rows, int hq, int hkv, int d, int max_rows, float scale, float softcap, int window,
+                  const void* out, int64_t ldo) {
+    return q && out && aligned(q, 16) && aligned(out, 16) && ldq % 8 == 0 && ldo % 8 == 0 && rows >= 0 && hq > 0 && hq <= 4096 &&
+           hkv > 0 && hq % hkv == 0 && ldq >= (int64_t)hq * d && ldo >= (int64_t)hq * d && max_rows > 0 && scale > 0.f && scale < INFINITY &&
+           softcap >= 0.f && softcap < INFINITY && window >= 0 && (int64_t)max_rows * (hq / hkv) < (1 << 30);
+}
+
+size_t attend_ws(int hq, int hkv, int d, int max_rows) {
+    const int64_t rows = (int64_t)max_rows * (hq / hkv);
+    return kMaxCtas * (sizeof(Desc) + 2 * (size_t)row_tiles(rows) * 8 * (d + 2) * sizeof(float));
+}
+
+int attend(const void* q, int64_t ldq, int rows, int hq, const void* k_pages, const void* v_pages, int64_t k_stride, int64_t v_stride,
+           int pages, int page, int hkv, int d, const int* table, int64_t ldt, int width, const int* lens, const int* cu, int batch,
+           int max_rows, float scale, float softcap, int window, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
+           void* stream) {
+    if (!kv_args_ok(k_pages, v_pages, k_stride, v_stride, pages, page, hkv, d, table, ldt, width, lens, cu, batch) ||
+        !attn_args_ok(q, ldq, rows, hq, hkv, d, max_rows, scale, softcap, window, out, ldo) || !workspace ||
+        !aligned(workspace, 16))
+        return B200Q_EINVAL;
+    if (workspace_bytes < attend_ws(hq, hkv, d, max_rows)) return B200Q_ENOSPACE;
+    if (rows == 0) return B200Q_OK;
+    AttnArgs a = {};
+    a.q = (const __nv_bfloat16*)q; a.ldq = ldq; a.rows = rows; a.out = (__nv_bfloat16*)out; a.ldo = ldo;
+    a.s = {table, lens, cu, ldt, width, batch};
+    a.max_rows = max_rows; a.hkv = hkv; a.group = hq / hkv; a.pages = pages; a.page_log2 = log2_of(page);
+    a.c = 1.4426950408889634f * (softcap > 0.f ? softcap : scale);
+    a.cap_in = softcap > 0.f ? scale / softcap : 0.f;
+    a.window = window > 0 && window < INT_MAX / 2 ? window : INT_MAX / 2;
+    a.ws = workspace;
+    CUtensorMap mk, mv;
+    if (!kv_tensor_map(&mk, k_pages, k_stride, pages, page, hkv, d, kUnit) ||
+        !kv_tensor_map(&mv, v_pages, v_stride, pages, page, hkv, d, kUnit))
+        return status_from(cudaErrorInvalidValue);
+    const cudaStream_t s = (cudaStream_t)stream;
+    const int nt = row_tiles((int64_t)max_rows * a.group);
+    cudaError_t e;
+    if (d == 128) e = nt == 1 ? launch_rows<128, 1>(mk, mv, a, s) : nt == 2 ? launch_rows<128, 2>(mk, mv, a, s) : launch_rows<128, 4>(mk, mv, a, s);
+    else e = nt == 1 ? launch_rows<64, 1>(mk, mv, a, s) : nt == 2 ? launch_rows<64, 2>(mk, mv, a, s) : launch_rows<64, 4>(mk, mv, a, s);
+    return status_from(e);
+}
+
+}  // namespace
+}  // namespace b200q
+
+using namespace b200q;
+
+extern "C" {
+
+size_t b200q_attn_decode_workspace_bytes(int hq, int hkv, int d, int max_rows) {
+    return hq <= 0 || hkv <= 0 || hq % hkv || max_rows <= 0 || max_rows > 16 ? 0 : attend_ws(hq, hkv, d, max_rows);
+}
+
+int b200q_attn_decode(const void* q, int64_t ldq, int rows, int hq, const void* k_pages, const void* v_pages, int64_t k_stride,
+                      int64_t v_stride, int pages, int page, int hkv, int d, const int* table, int64_t ldt, int width,
+                      const int* lens, const int* cu, int batch, int max_rows, float scale, float softcap, int window, void* out,
+                      int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
+    if (max_rows > 16) return B200Q_EINVAL;
+    return attend(q, ldq, rows, hq, k_pages, v_pages, k_stride, v_stride, pages, page, hkv, d, table, ldt, width, lens, cu, batch,
+                  max_rows, scale, softcap, window, out, ldo, workspace, workspace_bytes, stream);
+}
+
+size_t b200q_attn_prompt_workspace_bytes(int hq, int hkv, int d, int rows, int max_rows, int batch) {
+    (void)rows; (void)batch;
+    return hq <= 0 || hkv <= 0 || hq % hkv || max_rows <= 0 ? 0 : attend_ws(hq, hkv, d, max_rows);
+}
+
+int b200q_attn_prompt(const void* q, int64_t ldq, int rows, int hq, const void* k_pages, const void* v_pages, int64_t k_stride,
+                      int64_t v_stride, int pages, int page, int hkv, int d, const int* table, int64_t ldt, int width,
+                      const int* lens, const int* cu, int batch, int max_rows, float scale, float softcap, int window, void* out,
+                      int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
+    return attend(q, ldq, rows, hq, k_pages, v_pages, k_stride, v_stride, pages, page, hkv, d, table, ldt, width, lens, cu, batch,
+                  max_rows, scale, softcap, window, out, ldo, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

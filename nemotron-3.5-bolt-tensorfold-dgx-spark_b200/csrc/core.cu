@@ -22,6 +22,7 @@ __attribute__((weak)) int tc_error_read(int clear);     // tc_gemm.cu
 __attribute__((weak)) int nv4_error_read(int clear);    // nv4_gemm.cu
 __attribute__((weak)) int gemv_error_read(int clear);   // gemv_tc.cu
 __attribute__((weak)) int kv_error_read(int clear);     // kv.cu
+__attribute__((weak)) int attn_error_read(int clear);   // attn_decode.cu
 
 }  // namespace b200q
 
@@ -43,7 +44,7 @@ const char* b200q_strerror(int status) {
 
 int b200q_device_error(int clear) {
     int (*const read[])(int) = {iq2_error_read, tc_error_read, nv4_error_read, gemv_error_read,
-                                 kv_error_read};   // 4 bits each
+                                 kv_error_read, attn_error_read};   // 4 bits each
     int v = 0;
     for (int i = 0; i < (int)(sizeof(read) / sizeof(read[0])); i++) {
         const int e = read[i] ? read[i](clear) : 0;

@@ -41,11 +41,42 @@ def test_append_of_no_rows_is_nothing():
     assert b200q.lib().b200q_kv_append(*append_args(rows=0)) == b200q.OK
 
 
+def attn_args(**kw):
+    a = dict(q=vp(A), ldq=512, rows=4, hq=4, kp=vp(A), vp_=vp(A), ks=2 * 16 * 128, vs=2 * 16 * 128, pages=8, page=16, hkv=2, d=128,
+             table=vp(A), ldt=4, width=4, lens=vp(A), cu=vp(A), batch=2, max_rows=4, scale=0.1, softcap=0.0, window=0, out=vp(A),
+             ldo=512, ws=vp(A), wsb=1 << 40, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("f", ["b200q_attn_decode", "b200q_attn_prompt"])
+@pytest.mark.parametrize("kw", CACHE_REFUSALS + [
+    dict(q=None), dict(out=None), dict(q=vp(A + 8)), dict(out=vp(A + 4)), dict(ldq=504), dict(ldo=516), dict(rows=-1), dict(hq=0),
+    dict(hq=5), dict(max_rows=0), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
+    dict(softcap=-1.0), dict(softcap=float("nan")), dict(window=-1), dict(ws=None), dict(ws=vp(A + 8))])
+def test_attention_refuses(f, kw):
+    assert getattr(b200q.lib(), f)(*attn_args(**kw)) == b200q.EINVAL
+
+
+def test_attention_of_no_rows_too_many_and_too_little_workspace():
+    L = b200q.lib()
+    for f in (L.b200q_attn_decode, L.b200q_attn_prompt):
+        assert f(*attn_args(rows=0)) == b200q.OK
+        assert f(*attn_args(wsb=16)) == b200q.ENOSPACE
+    assert L.b200q_attn_decode(*attn_args(max_rows=17)) == b200q.EINVAL
+    assert L.b200q_attn_decode_workspace_bytes(4, 2, 128, 17) == 0
+    assert 0 < L.b200q_attn_decode_workspace_bytes(32, 8, 128, 1) <= 8 << 20
+
+
 def test_host_tensors_are_refused():
     step = Step([(1, 3)], 4, 2, 64, 16)
     x = torch.zeros(1, 4, 64)
     with pytest.raises(b200q.B200QError, match="CUDA tensor"):
         b200q.k_kv_append(x, x[:, :2], x[:, :2], *step.args())
+    for f in (b200q.attn_decode, b200q.attn_prompt):
+        with pytest.raises(b200q.B200QError, match="CUDA tensor"):
+            f(x.bfloat16(), *step.args(), 1)
 
 
 def test_the_rotation_is_a_complex_product():
