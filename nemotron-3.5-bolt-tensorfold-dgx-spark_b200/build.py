@@ -26,7 +26,7 @@ FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxe
 
 
 # the sources that neither read the IQ2_XXS tables nor call code that does
-TABLE_FREE = ("attn_decode.cu", "core.cu", "gemv_tc.cu", "kv.cu", "nv4_gemm.cu")
+TABLE_FREE = ("attn_decode.cu", "attn_prompt.cu", "core.cu", "gemv_tc.cu", "kv.cu", "nv4_gemm.cu")
 
 
 def sources():

@@ -1,5 +1,8 @@
 // Shared pieces of the paged attention kernels: their arguments, the score's scaling, the cache's tensor maps.
 #pragma once
+#include <climits>
+#include <cmath>
+
 #include <cuda.h>   // CUtensorMap and its enums: types alone, the encoder is looked up at run time
 
 #include "kv.cuh"
@@ -42,8 +45,27 @@ __device__ __forceinline__ void tma_kv(uint32_t dst, const CUtensorMap* m, int r
         ::"r"(dst), "l"(m), "r"(0), "r"(row), "r"(head), "r"(page), "r"(bar) : "memory");
 }
 
-// the tensor map of one side of the cache: dims (64, page, d / 64, heads, pages), box (64, box_rows, d / 64, 1, 1)
-bool kv_tensor_map(CUtensorMap* m, const void* base, int64_t page_stride, int pages, int page, int heads, int d, int box_rows);
+// the tensor map of one side of the cache: dims (64, page, d / 64, heads, pages), box (64, box_rows, box_blocks, 1, 1)
+bool kv_tensor_map(CUtensorMap* m, const void* base, int64_t page_stride, int pages, int page, int heads, int d, int box_rows,
+                   int box_blocks);
 int attn_sms();   // SMs of the current device
+
+inline bool attn_args_ok(const void* q, int64_t ldq, int rows, int hq, int hkv, int d, int max_rows, float scale, float softcap,
+                         int window, const void* out, int64_t ldo) {
+    return q && out && aligned(q, 16) && aligned(out, 16) && ldq % 8 == 0 && ldo % 8 == 0 && rows >= 0 && hq > 0 && hq <= 4096 &&
+           hkv > 0 && hq % hkv == 0 && ldq >= (int64_t)hq * d && ldo >= (int64_t)hq * d && max_rows > 0 && scale > 0.f &&
+           scale < INFINITY && softcap >= 0.f && softcap < INFINITY && window >= 0 && (int64_t)max_rows * (hq / hkv) < (1 << 30);
+}
+inline AttnArgs attn_args(const void* q, int64_t ldq, int rows, int hq, int hkv, int pages, int page, const KvSeqs& s, int max_rows,
+                          float scale, float softcap, int window, void* out, int64_t ldo, void* ws) {
+    AttnArgs a = {};
+    a.q = (const __nv_bfloat16*)q; a.ldq = ldq; a.rows = rows; a.out = (__nv_bfloat16*)out; a.ldo = ldo; a.s = s;
+    a.max_rows = max_rows; a.hkv = hkv; a.group = hq / hkv; a.pages = pages; a.page_log2 = log2_of(page);
+    a.c = 1.4426950408889634f * (softcap > 0.f ? softcap : scale);
+    a.cap_in = softcap > 0.f ? scale / softcap : 0.f;
+    a.window = window > 0 && window < INT_MAX / 2 ? window : INT_MAX / 2;
+    a.ws = ws;
+    return a;
+}
 
 }  // namespace b200q

@@ -19,8 +19,6 @@
 #include "attn.cuh"
 #include "tcgen05.cuh"
 
-#include <climits>
-
 namespace b200q {
 
 __device__ int g_attn_error;   // bit 0: a wait ran out, bit 1: a page table or length out of range, bit 2: over max_rows
@@ -48,7 +46,8 @@ int attn_sms() {
     return sms[dev];
 }
 
-bool kv_tensor_map(CUtensorMap* m, const void* base, int64_t page_stride, int pages, int page, int heads, int d, int box_rows) {
+bool kv_tensor_map(CUtensorMap* m, const void* base, int64_t page_stride, int pages, int page, int heads, int d, int box_rows,
+                   int box_blocks) {
     typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -63,7 +62,7 @@ bool kv_tensor_map(CUtensorMap* m, const void* base, int64_t page_stride, int pa
     if (!encode) return false;
     const cuuint64_t dims[5] = {64, (cuuint64_t)page, (cuuint64_t)d / 64, (cuuint64_t)heads, (cuuint64_t)pages};
     const cuuint64_t strides[4] = {(cuuint64_t)d * 2, 128, (cuuint64_t)page * d * 2, (cuuint64_t)page_stride * 2};
-    const cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)d / 64, 1, 1}, one[5] = {1, 1, 1, 1, 1};
+    const cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_blocks, 1, 1}, one[5] = {1, 1, 1, 1, 1};
     return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, one,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -576,46 +575,9 @@ cudaError_t launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const Attn
 
 int row_tiles(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
-bool attn_args_ok(const void* q, int64_t ldq, int rows, int hq, int hkv, int d, int max_rows, float scale, float softcap, int window,
-                  const void* out, int64_t ldo) {
-    return q && out && aligned(q, 16) && aligned(out, 16) && ldq % 8 == 0 && ldo % 8 == 0 && rows >= 0 && hq > 0 && hq <= 4096 &&
-           hkv > 0 && hq % hkv == 0 && ldq >= (int64_t)hq * d && ldo >= (int64_t)hq * d && max_rows > 0 && scale > 0.f && scale < INFINITY &&
-           softcap >= 0.f && softcap < INFINITY && window >= 0 && (int64_t)max_rows * (hq / hkv) < (1 << 30);
-}
-
 size_t attend_ws(int hq, int hkv, int d, int max_rows) {
     const int64_t rows = (int64_t)max_rows * (hq / hkv);
     return kMaxCtas * (sizeof(Desc) + 2 * (size_t)row_tiles(rows) * 8 * (d + 2) * sizeof(float));
-}
-
-int attend(const void* q, int64_t ldq, int rows, int hq, const void* k_pages, const void* v_pages, int64_t k_stride, int64_t v_stride,
-           int pages, int page, int hkv, int d, const int* table, int64_t ldt, int width, const int* lens, const int* cu, int batch,
-           int max_rows, float scale, float softcap, int window, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
-           void* stream) {
-    if (!kv_args_ok(k_pages, v_pages, k_stride, v_stride, pages, page, hkv, d, table, ldt, width, lens, cu, batch) ||
-        !attn_args_ok(q, ldq, rows, hq, hkv, d, max_rows, scale, softcap, window, out, ldo) || !workspace ||
-        !aligned(workspace, 16))
-        return B200Q_EINVAL;
-    if (workspace_bytes < attend_ws(hq, hkv, d, max_rows)) return B200Q_ENOSPACE;
-    if (rows == 0) return B200Q_OK;
-    AttnArgs a = {};
-    a.q = (const __nv_bfloat16*)q; a.ldq = ldq; a.rows = rows; a.out = (__nv_bfloat16*)out; a.ldo = ldo;
-    a.s = {table, lens, cu, ldt, width, batch};
-    a.max_rows = max_rows; a.hkv = hkv; a.group = hq / hkv; a.pages = pages; a.page_log2 = log2_of(page);
-    a.c = 1.4426950408889634f * (softcap > 0.f ? softcap : scale);
-    a.cap_in = softcap > 0.f ? scale / softcap : 0.f;
-    a.window = window > 0 && window < INT_MAX / 2 ? window : INT_MAX / 2;
-    a.ws = workspace;
-    CUtensorMap mk, mv;
-    if (!kv_tensor_map(&mk, k_pages, k_stride, pages, page, hkv, d, kUnit) ||
-        !kv_tensor_map(&mv, v_pages, v_stride, pages, page, hkv, d, kUnit))
-        return status_from(cudaErrorInvalidValue);
-    const cudaStream_t s = (cudaStream_t)stream;
-    const int nt = row_tiles((int64_t)max_rows * a.group);
-    cudaError_t e;
-    if (d == 128) e = nt == 1 ? launch_rows<128, 1>(mk, mv, a, s) : nt == 2 ? launch_rows<128, 2>(mk, mv, a, s) : launch_rows<128, 4>(mk, mv, a, s);
-    else e = nt == 1 ? launch_rows<64, 1>(mk, mv, a, s) : nt == 2 ? launch_rows<64, 2>(mk, mv, a, s) : launch_rows<64, 4>(mk, mv, a, s);
-    return status_from(e);
 }
 
 }  // namespace
@@ -633,22 +595,24 @@ int b200q_attn_decode(const void* q, int64_t ldq, int rows, int hq, const void* 
                       int64_t v_stride, int pages, int page, int hkv, int d, const int* table, int64_t ldt, int width,
                       const int* lens, const int* cu, int batch, int max_rows, float scale, float softcap, int window, void* out,
                       int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
-    if (max_rows > 16) return B200Q_EINVAL;
-    return attend(q, ldq, rows, hq, k_pages, v_pages, k_stride, v_stride, pages, page, hkv, d, table, ldt, width, lens, cu, batch,
-                  max_rows, scale, softcap, window, out, ldo, workspace, workspace_bytes, stream);
-}
-
-size_t b200q_attn_prompt_workspace_bytes(int hq, int hkv, int d, int rows, int max_rows, int batch) {
-    (void)rows; (void)batch;
-    return hq <= 0 || hkv <= 0 || hq % hkv || max_rows <= 0 ? 0 : attend_ws(hq, hkv, d, max_rows);
-}
-
-int b200q_attn_prompt(const void* q, int64_t ldq, int rows, int hq, const void* k_pages, const void* v_pages, int64_t k_stride,
-                      int64_t v_stride, int pages, int page, int hkv, int d, const int* table, int64_t ldt, int width,
-                      const int* lens, const int* cu, int batch, int max_rows, float scale, float softcap, int window, void* out,
-                      int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
-    return attend(q, ldq, rows, hq, k_pages, v_pages, k_stride, v_stride, pages, page, hkv, d, table, ldt, width, lens, cu, batch,
-                  max_rows, scale, softcap, window, out, ldo, workspace, workspace_bytes, stream);
+    if (!kv_args_ok(k_pages, v_pages, k_stride, v_stride, pages, page, hkv, d, table, ldt, width, lens, cu, batch) ||
+        !attn_args_ok(q, ldq, rows, hq, hkv, d, max_rows, scale, softcap, window, out, ldo) || max_rows > 16 || !workspace ||
+        !aligned(workspace, 16))
+        return B200Q_EINVAL;
+    if (workspace_bytes < attend_ws(hq, hkv, d, max_rows)) return B200Q_ENOSPACE;
+    if (rows == 0) return B200Q_OK;
+    const AttnArgs a = attn_args(q, ldq, rows, hq, hkv, pages, page, {table, lens, cu, ldt, width, batch}, max_rows, scale, softcap, window,
+                                 out, ldo, workspace);
+    CUtensorMap mk, mv;
+    if (!kv_tensor_map(&mk, k_pages, k_stride, pages, page, hkv, d, kUnit, d / 64) ||
+        !kv_tensor_map(&mv, v_pages, v_stride, pages, page, hkv, d, kUnit, d / 64))
+        return status_from(cudaErrorInvalidValue);
+    const cudaStream_t s = (cudaStream_t)stream;
+    const int nt = row_tiles((int64_t)max_rows * a.group);
+    cudaError_t e;
+    if (d == 128) e = nt == 1 ? launch_rows<128, 1>(mk, mv, a, s) : nt == 2 ? launch_rows<128, 2>(mk, mv, a, s) : launch_rows<128, 4>(mk, mv, a, s);
+    else e = nt == 1 ? launch_rows<64, 1>(mk, mv, a, s) : nt == 2 ? launch_rows<64, 2>(mk, mv, a, s) : launch_rows<64, 4>(mk, mv, a, s);
+    return status_from(e);
 }
 
 }  // extern "C"

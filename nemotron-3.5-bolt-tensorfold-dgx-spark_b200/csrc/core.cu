@@ -23,6 +23,7 @@ __attribute__((weak)) int nv4_error_read(int clear);    // nv4_gemm.cu
 __attribute__((weak)) int gemv_error_read(int clear);   // gemv_tc.cu
 __attribute__((weak)) int kv_error_read(int clear);     // kv.cu
 __attribute__((weak)) int attn_error_read(int clear);   // attn_decode.cu
+__attribute__((weak)) int prompt_error_read(int clear); // attn_prompt.cu
 
 }  // namespace b200q
 
@@ -43,13 +44,14 @@ const char* b200q_strerror(int status) {
 }
 
 int b200q_device_error(int clear) {
-    int (*const read[])(int) = {iq2_error_read, tc_error_read, nv4_error_read, gemv_error_read,
-                                 kv_error_read, attn_error_read};   // 4 bits each
+    const struct { int (*read)(int); int shift; } words[] = {
+        {iq2_error_read, 0}, {tc_error_read, 4}, {nv4_error_read, 8}, {gemv_error_read, 12}, {kv_error_read, 16},
+        {attn_error_read, 20}, {prompt_error_read, 20}};   // both forms of the paged attention report alike
     int v = 0;
-    for (int i = 0; i < (int)(sizeof(read) / sizeof(read[0])); i++) {
-        const int e = read[i] ? read[i](clear) : 0;
+    for (const auto& w : words) {
+        const int e = w.read ? w.read(clear) : 0;
         if (e < 0) return -1;
-        v |= e << (4 * i);
+        v |= e << w.shift;
     }
     return v;
 }
