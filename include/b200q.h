@@ -334,9 +334,19 @@ int b200q_moe_decode_noalloc(const void* x, const void* logits, const void* up, 
  * own included, so its row i of r stands at position lens[b] - r + i; the token at position p lives in page
  * table[b * ldt + p / page], row p % page.  cu [batch + 1], lens [batch] and table [batch][ldt >= width] are int32 on the
  * device, read by the kernels alone: a captured graph follows their contents.  Rows outside cu[0] .. cu[batch] - 1
- * (padding) are neither read nor written, nor are rows at a negative position.  batch <= 4096,
- * width * page <= 2^30.
+ * (padding) are neither read nor written.  batch <= 4096, width * page <= 2^30.
  * --------------------------------------------------------------------------------------------------------- */
+typedef struct b200q_paged {
+    const void* k_pages;   /* bf16; written by b200q_kv_append alone */
+    const void* v_pages;
+    int64_t k_stride, v_stride;
+    const int* table;
+    const int* lens;
+    const int* cu;
+    int64_t ldt;
+    int pages, page, hkv, d;
+    int width, batch;
+} b200q_paged;
 
 /* Append (the role of kv_store_k, bolt_kernels.cu:1735, with the steps before it): for each of `rows` rows
  *   q_out = bf16(rotate(norm(q))),  k_pages[slot] = bf16(rotate(norm(k))),  v_pages[slot] = bf16(v)
@@ -346,13 +356,13 @@ int b200q_moe_decode_noalloc(const void* x, const void* logits, const void* up, 
  * norm: x * rsqrt(mean(x^2) + eps) * w over each head, w = q_norm / k_norm [d] (norm_dtype fp32 or bf16), NULL: none.
  * rotate: the first `rope` values of a head (a multiple of 16, 0: none) in pairs (i, i + rope / 2), or (2i, 2i + 1) when
  * interleaved, by the angle position * inv_freq[i] (fp32 [rope / 2]).
- * A row whose position has no table entry, or whose entry is no page of the cache, gets q_out but stores nothing, and sets
- * bit 16 of b200q_device_error.  Two rows of a call must not name the same slot.  Pointers 16-byte aligned. */
-int b200q_kv_append(const void* q, const void* k, const void* v, int x_dtype, int64_t ldq, int64_t ldk, int64_t ldv,
-                    int rows, int hq, int hkv, int d, void* k_pages, void* v_pages, int64_t k_stride, int64_t v_stride,
-                    int pages, int page, const int* table, int64_t ldt, int width, const int* lens, const int* cu,
-                    int batch, const float* inv_freq, int rope, int interleaved, const void* q_norm, const void* k_norm,
-                    int norm_dtype, float eps, void* q_out, int64_t ldo, void* stream);
+ * A row at a negative position is left alone like padding.  A row whose position has no table entry, or whose entry is
+ * no page of the cache, gets q_out but stores nothing, and sets bit 16 of b200q_device_error.  Two rows of a call must
+ * not name the same slot.  Pointers 16-byte aligned. */
+int b200q_kv_append(const b200q_paged* kv, const void* q, const void* k, const void* v, int x_dtype, int64_t ldq,
+                    int64_t ldk, int64_t ldv, int rows, int hq, const float* inv_freq, int rope, int interleaved,
+                    const void* q_norm, const void* k_norm, int norm_dtype, float eps, void* q_out, int64_t ldo,
+                    void* stream);
 
 /* Attention over the cache (the roles of attn_part_k / attn_blk_part_k, bolt_kernels.cu:1779-2009, and attn_mma_part_k /
  * attn_mma2_part_k, bolt_mma.cu:1406-1724, with their combines): for each row of the step and query head h
@@ -367,15 +377,11 @@ int b200q_kv_append(const void* q, const void* k, const void* v, int x_dtype, in
  * workspace: >= the *_workspace_bytes query, 16-byte aligned, contents of no matter before and after a call; two calls
  * that may overlap need one each. */
 size_t b200q_attn_decode_workspace_bytes(int hq, int hkv, int d, int max_rows);
-int b200q_attn_decode(const void* q, int64_t ldq, int rows, int hq, const void* k_pages, const void* v_pages,
-                      int64_t k_stride, int64_t v_stride, int pages, int page, int hkv, int d, const int* table,
-                      int64_t ldt, int width, const int* lens, const int* cu, int batch, int max_rows, float scale,
+int b200q_attn_decode(const b200q_paged* kv, const void* q, int64_t ldq, int rows, int hq, int max_rows, float scale,
                       float softcap, int window, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
                       void* stream);
 size_t b200q_attn_prompt_workspace_bytes(int hq, int hkv, int d, int rows, int max_rows, int batch);
-int b200q_attn_prompt(const void* q, int64_t ldq, int rows, int hq, const void* k_pages, const void* v_pages,
-                      int64_t k_stride, int64_t v_stride, int pages, int page, int hkv, int d, const int* table,
-                      int64_t ldt, int width, const int* lens, const int* cu, int batch, int max_rows, float scale,
+int b200q_attn_prompt(const b200q_paged* kv, const void* q, int64_t ldq, int rows, int hq, int max_rows, float scale,
                       float softcap, int window, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
                       void* stream);
 

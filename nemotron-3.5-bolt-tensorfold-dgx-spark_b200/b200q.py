@@ -9,8 +9,10 @@ every operator raises.
 """
 import contextlib
 import ctypes
+import functools
 import json
 import os
+import struct
 
 import torch
 
@@ -95,14 +97,12 @@ def lib():
             "b200q_quant_nv4_rows": (i32, [vp, i32, i32, i32, i32, vp, vp]),
             "b200q_nv4_gemm_workspace_bytes": (sz, [i32, i32, i32]),
             "b200q_nv4_gemm": (i32, [vp, i32, i32, f32, vp, i32, vp, i32, vp, sz, vp]),
-            "b200q_kv_append": (i32, [vp, vp, vp, i32, i64, i64, i64, i32, i32, i32, i32, vp, vp, i64, i64, i32, i32, vp, i64,
-                                      i32, vp, vp, i32, vp, i32, i32, vp, vp, i32, f32, vp, i64, vp]),
+            "b200q_kv_append": (i32, [ctypes.c_char_p, vp, vp, vp, i32, i64, i64, i64, i32, i32, vp, i32, i32, vp, vp, i32,
+                                      f32, vp, i64, vp]),
             "b200q_attn_decode_workspace_bytes": (sz, [i32, i32, i32, i32]),
-            "b200q_attn_decode": (i32, [vp, i64, i32, i32, vp, vp, i64, i64, i32, i32, i32, i32, vp, i64, i32, vp, vp, i32,
-                                        i32, f32, f32, i32, vp, i64, vp, sz, vp]),
+            "b200q_attn_decode": (i32, [ctypes.c_char_p, vp, i64, i32, i32, i32, f32, f32, i32, vp, i64, vp, sz, vp]),
             "b200q_attn_prompt_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
-            "b200q_attn_prompt": (i32, [vp, i64, i32, i32, vp, vp, i64, i64, i32, i32, i32, i32, vp, i64, i32, vp, vp, i32,
-                                        i32, f32, f32, i32, vp, i64, vp, sz, vp]),
+            "b200q_attn_prompt": (i32, [ctypes.c_char_p, vp, i64, i32, i32, i32, f32, f32, i32, vp, i64, vp, sz, vp]),
             "b200q_ckpt_open": (vp, [ctypes.c_char_p]),
             "b200q_ckpt_close": (None, [vp]),
             "b200q_ckpt_count": (i64, [vp]),
@@ -566,58 +566,71 @@ def moe_prompt(up, down, E, H, F, counts, offsets, order, topk, x, mo=None, act=
 
 # -------------------------------------------------------------------------------------------------------------
 # paged attention (kv_store and the attention between the q/k/v projection and o_proj)
+#
+# A decode step makes three of these calls a layer with a few microseconds of work each, so their checks read every tensor
+# attribute once.
 # -------------------------------------------------------------------------------------------------------------
-def _heads(t, name, device, dtype=None):
-    """rows of heads [rows][heads][d] on `device`, a row's heads contiguous, rows at any pitch -> its pitch"""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda):
-        raise B200QError(EINVAL, f"{name} must be a CUDA tensor")
-    if t.device != device:
-        raise B200QError(EINVAL, f"{name} is on {t.device}, the cache on {device}")
-    if dtype is not None and t.dtype != dtype:
-        raise B200QError(EINVAL, f"{name} must be {dtype}")
-    if t.dim() != 3:
-        raise B200QError(EINVAL, f"{name} must be [rows][heads][d]")
-    n, h, d = t.shape
-    s0, s1, s2 = t.stride()
-    if n * h * d and ((s2 != 1 and d > 1) or (s1 != d and h > 1)):
-        raise B200QError(EINVAL, f"{name}'s heads must be contiguous in a row")
-    return s0 if n > 1 else h * d
+_PAGED = struct.Struct("PPqqPPPqiiiiii")   # b200q_paged
+
+
+def _all_on(dev, *tensors):
+    """whether all are tensors on CUDA device `dev`"""
+    try:
+        for t in tensors:
+            if t.get_device() != dev:
+                return False
+    except AttributeError:
+        return False
+    return dev >= 0
 
 
 def _paged(k_pages, v_pages, table, lens, cu):
-    """the cache and the step's description, checked -> the C ABI's arguments
-    (k_pages, v_pages, k_stride, v_stride, pages, page), (table, ldt, width, lens, cu, batch)"""
-    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages"), (table, "table"), (lens, "lens"), (cu, "cu")):
-        if not (isinstance(t, torch.Tensor) and t.is_cuda):
-            raise B200QError(EINVAL, f"{name} must be a CUDA tensor")
-        if t.device != k_pages.device:
-            raise B200QError(EINVAL, f"{name} is on {t.device}, the cache on {k_pages.device}")
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != torch.bfloat16 or \
-            v_pages.dtype != torch.bfloat16:
+    """the cache and the step's description, checked -> (b200q_paged's bytes, device index, hkv, d, batch)"""
+    dev = k_pages.get_device() if isinstance(k_pages, torch.Tensor) else -1
+    if not _all_on(dev, v_pages, table, lens, cu):
+        raise B200QError(EINVAL, "k_pages, v_pages, table, lens and cu must be CUDA tensors on one device")
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or k_pages.dtype is not torch.bfloat16 or \
+            v_pages.dtype is not torch.bfloat16:
         raise B200QError(EINVAL, "k_pages and v_pages must be bf16 [pages][heads][page][d] of one shape")
-    pages, h, page, d = k_pages.shape
-    inner = (page * d, d, 1)
-    if pages * h * page * d == 0 or k_pages.stride()[1:] != inner or v_pages.stride()[1:] != inner:
-        raise B200QError(EINVAL, "a page of the cache must be contiguous and not empty")
-    if table.dim() != 2 or table.dtype != torch.int32 or lens.dim() != 1 or lens.dtype != torch.int32 or cu.dim() != 1 or \
-            cu.dtype != torch.int32:
-        raise B200QError(EINVAL, "table [batch][pages], lens [batch] and cu [batch + 1] must be int32")
-    batch, width = table.shape
-    if batch == 0 or width == 0 or table.stride(1) != 1 or lens.shape[0] != batch or cu.shape[0] != batch + 1 or \
-            lens.stride(0) != 1 or cu.stride(0) != 1:
-        raise B200QError(EINVAL, "table [batch][pages], lens [batch] and cu [batch + 1] must be contiguous and agree")
+    pages, h, page, d = shape
     one = h * page * d
-    return ((k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0) if pages > 1 else one,
-             v_pages.stride(0) if pages > 1 else one, pages, page),
-            (table.data_ptr(), table.stride(0) if batch > 1 else width, width, lens.data_ptr(), cu.data_ptr(), batch))
+    ks, k1, k2, k3 = k_pages.stride()
+    vs, v1, v2, v3 = v_pages.stride()
+    if not pages * one or k3 != 1 or v3 != 1 or k2 != d or v2 != d or ((k1 != page * d or v1 != page * d) and h > 1):
+        raise B200QError(EINVAL, "a page of the cache must be contiguous and not empty")
+    shape, i32 = table.shape, torch.int32
+    batch, width = shape if len(shape) == 2 else (0, 0)
+    if not batch or not width or table.dtype is not i32 or lens.dtype is not i32 or cu.dtype is not i32 or \
+            lens.shape != (batch,) or cu.shape != (batch + 1,):
+        raise B200QError(EINVAL, "table [batch][pages], lens [batch] and cu [batch + 1] must be int32 and agree")
+    ldt, t1 = table.stride()
+    if (t1 != 1 and width > 1) or not cu.is_contiguous() or not lens.is_contiguous():
+        raise B200QError(EINVAL, "rows of table, lens and cu must be contiguous")
+    return (_PAGED.pack(k_pages.data_ptr(), v_pages.data_ptr(), ks if pages > 1 else one, vs if pages > 1 else one,
+                        table.data_ptr(), lens.data_ptr(), cu.data_ptr(), ldt if batch > 1 else width, pages, page, h, d, width,
+                        batch), dev, h, d, batch)
+
+
+def _heads(t, name, dev, dtype, d):
+    """[rows][heads][d] of `dtype` on device `dev`, a row's heads contiguous, rows at any pitch -> rows, heads, pitch"""
+    if not _all_on(dev, t):
+        raise B200QError(EINVAL, f"{name} must be a CUDA tensor on the cache's device")
+    shape, s = t.shape, t.stride()
+    if t.dtype is not dtype or len(shape) != 3 or shape[2] != d:
+        raise B200QError(EINVAL, f"{name} must be {dtype} [rows][heads][{d}]")
+    n, h = shape[0], shape[1]
+    if n and h and (s[2] != 1 or (s[1] != d and h > 1)):
+        raise B200QError(EINVAL, f"{name}'s heads must be contiguous in a row")
+    return n, h, s[0] if n > 1 else h * d
 
 
 _HERE = contextlib.nullcontext()
 
 
-def _on(device):
-    """a context in which `device` is the current one"""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _on(dev):
+    """a context in which device `dev` is the current one"""
+    return _HERE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def k_kv_append(q, k, v, k_pages, v_pages, table, lens, cu, inv_freq=None, interleaved=False, q_norm=None, k_norm=None,
@@ -628,75 +641,75 @@ def k_kv_append(q, k, v, k_pages, v_pages, table, lens, cu, inv_freq=None, inter
     projection's output); k_pages / v_pages [pages][hkv][page][d] bf16; table [batch][width], lens [batch],
     cu [batch + 1] int32; inv_freq: fp32 [rope / 2], rotates the first `rope` values of each query and key head;
     q_norm / k_norm [d]: weights of the RMS norm of each head.  -> q_out [rows][hq][d] bf16 (padding rows unwritten)"""
-    cache, seqs = _paged(k_pages, v_pages, table, lens, cu)
-    dev = k_pages.device
-    ldk, ldv = _heads(k, "k", dev), _heads(v, "v", dev, k.dtype)
-    hkv, d = k_pages.shape[1], k_pages.shape[3]
-    if k.shape != v.shape or k.shape[1:] != (hkv, d):
+    kv, dev, hkv, d, _ = _paged(k_pages, v_pages, table, lens, cu)
+    dt = k.dtype if isinstance(k, torch.Tensor) else None
+    if dt is not torch.float32 and dt is not torch.bfloat16:
+        raise B200QError(EINVAL, "q, k and v must be fp32 or bf16 CUDA tensors")
+    rows, hk, ldk = _heads(k, "k", dev, dt, d)
+    nv, hv, ldv = _heads(v, "v", dev, dt, d)
+    if nv != rows or hk != hkv or hv != hkv:
         raise B200QError(EINVAL, f"k and v must be [rows][{hkv}][{d}] like the cache")
-    rows, hq, ldq, ldo, qp, op = k.shape[0], 0, 0, 0, None, None
+    hq, ldq, ldo, qp, op = 0, 0, 0, None, None
     if q is not None:
-        ldq = _heads(q, "q", dev, k.dtype)
-        if q.shape[0] != rows or q.shape[2] != d:
-            raise B200QError(EINVAL, f"q must be [{rows}][heads][{d}]")
-        hq = q.shape[1]
+        nq, hq, ldq = _heads(q, "q", dev, dt, d)
         if q_out is None:
-            q_out = torch.empty(rows, hq, d, dtype=torch.bfloat16, device=dev)
-        ldo = _heads(q_out, "q_out", dev, torch.bfloat16)
-        if q_out.shape != q.shape:
-            raise B200QError(EINVAL, "q_out must have q's shape")
+            q_out = torch.empty(nq, hq, d, dtype=torch.bfloat16, device=k_pages.device)
+        no, ho, ldo = _heads(q_out, "q_out", dev, torch.bfloat16, d)
+        if nq != rows or no != rows or ho != hq:
+            raise B200QError(EINVAL, f"q and q_out must be [{rows}][heads][{d}]")
         qp, op = q.data_ptr(), q_out.data_ptr()
-    rope = 0
+    rope, fp = 0, None
     if inv_freq is not None:
-        if not (isinstance(inv_freq, torch.Tensor) and inv_freq.device == dev and inv_freq.dtype == torch.float32 and
-                inv_freq.dim() == 1 and inv_freq.is_contiguous()):
+        if not _all_on(dev, inv_freq) or inv_freq.dtype is not torch.float32 or not inv_freq.is_contiguous():
             raise B200QError(EINVAL, "inv_freq must be a contiguous fp32 CUDA tensor beside the cache")
-        rope = 2 * inv_freq.numel()
-    norm_dtype = F32
-    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if w is None:
-            continue
-        if not (isinstance(w, torch.Tensor) and w.device == dev and w.shape == (d,) and w.is_contiguous()):
-            raise B200QError(EINVAL, f"{name} must be a contiguous [{d}] CUDA tensor beside the cache")
-        norm_dtype = _dtype_code(w)
-    if q_norm is not None and k_norm is not None and q_norm.dtype != k_norm.dtype:
+        rope, fp = 2 * inv_freq.numel(), inv_freq.data_ptr()
+    norm_dtype, norms = F32, [None, None]
+    for i, w in enumerate((q_norm, k_norm)):
+        if w is not None:
+            if not _all_on(dev, w) or w.shape != (d,) or not w.is_contiguous():
+                raise B200QError(EINVAL, f"q_norm and k_norm must be contiguous [{d}] CUDA tensors beside the cache")
+            norm_dtype, norms[i] = _dtype_code(w), w.data_ptr()
+    if norms[0] and norms[1] and q_norm.dtype is not k_norm.dtype:
         raise B200QError(EINVAL, "q_norm and k_norm must have one dtype")
     if rows == 0:
         return q_out
     with _on(dev):
-        _check(lib().b200q_kv_append(qp, k.data_ptr(), v.data_ptr(), _dtype_code(k), ldq, ldk, ldv, rows, hq, hkv, d,
-                                     *cache, *seqs, inv_freq.data_ptr() if rope else None, rope, 1 if interleaved else 0,
-                                     _p(q_norm), _p(k_norm), norm_dtype, float(eps), op, ldo, _s()), "k_kv_append")
+        st = lib().b200q_kv_append(kv, qp, k.data_ptr(), v.data_ptr(), F32 if dt is torch.float32 else BF16, ldq, ldk, ldv, rows,
+                                   hq, fp, rope, 1 if interleaved else 0, norms[0], norms[1], norm_dtype, eps, op, ldo,
+                                   torch.cuda.current_stream().cuda_stream)
+    _check(st, "k_kv_append")
     return q_out
 
 
-def _attend(what, q, k_pages, v_pages, table, lens, cu, max_rows, scale, softcap, window, out):
-    cache, seqs = _paged(k_pages, v_pages, table, lens, cu)
-    dev = k_pages.device
-    hkv, d = k_pages.shape[1], k_pages.shape[3]
-    ldq = _heads(q, "q", dev, torch.bfloat16)
-    rows, hq = q.shape[:2]
-    if q.shape[2] != d or hq % hkv:
-        raise B200QError(EINVAL, f"q must be [rows][a multiple of {hkv}][{d}]")
+@functools.lru_cache(maxsize=1024)
+def _attn_workspace(name, dev, *sizes):
+    with _on(dev):   # the prompt form's depends on the device's SMs
+        return getattr(lib(), name)(*sizes)
+
+
+def _attend(name, q, k_pages, v_pages, table, lens, cu, max_rows, scale, softcap, window, out):
+    kv, dev, hkv, d, batch = _paged(k_pages, v_pages, table, lens, cu)
+    rows, hq, ldq = _heads(q, "q", dev, torch.bfloat16, d)
     if out is None:
-        out = torch.empty(rows, hq, d, dtype=torch.bfloat16, device=dev)
-    elif out.shape != q.shape:
-        raise B200QError(EINVAL, "out must have q's shape")
-    ldo = _heads(out, "out", dev, torch.bfloat16)
+        out = torch.empty(rows, hq, d, dtype=torch.bfloat16, device=k_pages.device)
+        ldo = hq * d
+    else:
+        no, ho, ldo = _heads(out, "out", dev, torch.bfloat16, d)
+        if no != rows or ho != hq:
+            raise B200QError(EINVAL, "out must have q's shape")
     if rows == 0:
         return out
-    L = lib()
     with _on(dev):
-        # scratch of this call alone: calls on other streams, and captured ones, have their own
-        if what == "attn_decode":
-            ws = torch.empty(L.b200q_attn_decode_workspace_bytes(hq, hkv, d, max_rows), dtype=torch.uint8, device=dev)
-            fn = L.b200q_attn_decode
+        if name == "attn_decode":
+            fn, nb = lib().b200q_attn_decode, _attn_workspace("b200q_attn_decode_workspace_bytes", dev, hq, hkv, d, max_rows)
         else:
-            ws = torch.empty(L.b200q_attn_prompt_workspace_bytes(hq, hkv, d, rows, max_rows, seqs[5]), dtype=torch.uint8,
-                             device=dev)
-            fn = L.b200q_attn_prompt
-        _check(fn(q.data_ptr(), ldq, rows, hq, *cache, hkv, d, *seqs, max_rows, d ** -0.5 if scale is None else scale, softcap,
-                  window, out.data_ptr(), ldo, ws.data_ptr(), ws.numel(), _s()), what)
+            fn, nb = lib().b200q_attn_prompt, _attn_workspace("b200q_attn_prompt_workspace_bytes", dev, hq, hkv, d, rows,
+                                                              max_rows, batch)
+        # scratch of this call alone: calls on other streams, and captured ones, have their own
+        ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=k_pages.device)
+        st = fn(kv, q.data_ptr(), ldq, rows, hq, max_rows, d ** -0.5 if scale is None else scale, softcap, window,
+                out.data_ptr(), ldo, ws.data_ptr(), nb, torch.cuda.current_stream().cuda_stream)
+    _check(st, name)
     return out
 
 

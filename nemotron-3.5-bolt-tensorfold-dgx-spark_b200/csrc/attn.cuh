@@ -46,21 +46,22 @@ __device__ __forceinline__ void tma_kv(uint32_t dst, const CUtensorMap* m, int r
 }
 
 // the tensor map of one side of the cache: dims (64, page, d / 64, heads, pages), box (64, box_rows, box_blocks, 1, 1)
-bool kv_tensor_map(CUtensorMap* m, const void* base, int64_t page_stride, int pages, int page, int heads, int d, int box_rows,
-                   int box_blocks);
+bool kv_tensor_map(CUtensorMap* m, const void* pages, int64_t stride, const b200q_paged& kv, int box_rows, int box_blocks);
 int attn_sms();   // SMs of the current device
 
-inline bool attn_args_ok(const void* q, int64_t ldq, int rows, int hq, int hkv, int d, int max_rows, float scale, float softcap,
-                         int window, const void* out, int64_t ldo) {
-    return q && out && aligned(q, 16) && aligned(out, 16) && ldq % 8 == 0 && ldo % 8 == 0 && rows >= 0 && hq > 0 && hq <= 4096 &&
-           hkv > 0 && hq % hkv == 0 && ldq >= (int64_t)hq * d && ldo >= (int64_t)hq * d && max_rows > 0 && scale > 0.f &&
-           scale < INFINITY && softcap >= 0.f && softcap < INFINITY && window >= 0 && (int64_t)max_rows * (hq / hkv) < (1 << 30);
+// the checks both forms share
+inline bool attn_ok(const b200q_paged* kv, const void* q, int64_t ldq, int rows, int hq, int max_rows, float scale, float softcap,
+                    int window, const void* out, int64_t ldo, const void* workspace) {
+    return kv_ok(kv) && q && out && workspace && aligned(q, 16) && aligned(out, 16) && aligned(workspace, 16) && ldq % 8 == 0 &&
+           ldo % 8 == 0 && rows >= 0 && hq > 0 && hq <= 4096 && hq % kv->hkv == 0 && ldq >= (int64_t)hq * kv->d &&
+           ldo >= (int64_t)hq * kv->d && max_rows > 0 && (int64_t)max_rows * (hq / kv->hkv) < (1 << 30) && scale > 0.f &&
+           scale < INFINITY && softcap >= 0.f && softcap < INFINITY && window >= 0;
 }
-inline AttnArgs attn_args(const void* q, int64_t ldq, int rows, int hq, int hkv, int pages, int page, const KvSeqs& s, int max_rows,
-                          float scale, float softcap, int window, void* out, int64_t ldo, void* ws) {
+inline AttnArgs attn_args(const b200q_paged& kv, const void* q, int64_t ldq, int rows, int hq, int max_rows, float scale, float softcap,
+                          int window, void* out, int64_t ldo, void* ws) {
     AttnArgs a = {};
-    a.q = (const __nv_bfloat16*)q; a.ldq = ldq; a.rows = rows; a.out = (__nv_bfloat16*)out; a.ldo = ldo; a.s = s;
-    a.max_rows = max_rows; a.hkv = hkv; a.group = hq / hkv; a.pages = pages; a.page_log2 = log2_of(page);
+    a.q = (const __nv_bfloat16*)q; a.ldq = ldq; a.rows = rows; a.out = (__nv_bfloat16*)out; a.ldo = ldo; a.s = kv_seqs(kv);
+    a.max_rows = max_rows; a.hkv = kv.hkv; a.group = hq / kv.hkv; a.pages = kv.pages; a.page_log2 = log2_of(kv.page);
     a.c = 1.4426950408889634f * (softcap > 0.f ? softcap : scale);
     a.cap_in = softcap > 0.f ? scale / softcap : 0.f;
     a.window = window > 0 && window < INT_MAX / 2 ? window : INT_MAX / 2;

@@ -46,8 +46,7 @@ int attn_sms() {
     return sms[dev];
 }
 
-bool kv_tensor_map(CUtensorMap* m, const void* base, int64_t page_stride, int pages, int page, int heads, int d, int box_rows,
-                   int box_blocks) {
+bool kv_tensor_map(CUtensorMap* m, const void* pages, int64_t stride, const b200q_paged& kv, int box_rows, int box_blocks) {
     typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -60,10 +59,10 @@ bool kv_tensor_map(CUtensorMap* m, const void* base, int64_t page_stride, int pa
         return (Encode)f;
     }();
     if (!encode) return false;
-    const cuuint64_t dims[5] = {64, (cuuint64_t)page, (cuuint64_t)d / 64, (cuuint64_t)heads, (cuuint64_t)pages};
-    const cuuint64_t strides[4] = {(cuuint64_t)d * 2, 128, (cuuint64_t)page * d * 2, (cuuint64_t)page_stride * 2};
+    const cuuint64_t dims[5] = {64, (cuuint64_t)kv.page, (cuuint64_t)kv.d / 64, (cuuint64_t)kv.hkv, (cuuint64_t)kv.pages};
+    const cuuint64_t strides[4] = {(cuuint64_t)kv.d * 2, 128, (cuuint64_t)kv.page * kv.d * 2, (cuuint64_t)stride * 2};
     const cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_blocks, 1, 1}, one[5] = {1, 1, 1, 1, 1};
-    return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, one,
+    return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(pages), dims, strides, box, one,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -591,21 +590,16 @@ size_t b200q_attn_decode_workspace_bytes(int hq, int hkv, int d, int max_rows) {
     return hq <= 0 || hkv <= 0 || hq % hkv || max_rows <= 0 || max_rows > 16 ? 0 : attend_ws(hq, hkv, d, max_rows);
 }
 
-int b200q_attn_decode(const void* q, int64_t ldq, int rows, int hq, const void* k_pages, const void* v_pages, int64_t k_stride,
-                      int64_t v_stride, int pages, int page, int hkv, int d, const int* table, int64_t ldt, int width,
-                      const int* lens, const int* cu, int batch, int max_rows, float scale, float softcap, int window, void* out,
-                      int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!kv_args_ok(k_pages, v_pages, k_stride, v_stride, pages, page, hkv, d, table, ldt, width, lens, cu, batch) ||
-        !attn_args_ok(q, ldq, rows, hq, hkv, d, max_rows, scale, softcap, window, out, ldo) || max_rows > 16 || !workspace ||
-        !aligned(workspace, 16))
-        return B200Q_EINVAL;
-    if (workspace_bytes < attend_ws(hq, hkv, d, max_rows)) return B200Q_ENOSPACE;
+int b200q_attn_decode(const b200q_paged* kv, const void* q, int64_t ldq, int rows, int hq, int max_rows, float scale, float softcap,
+                      int window, void* out, int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!attn_ok(kv, q, ldq, rows, hq, max_rows, scale, softcap, window, out, ldo, workspace) || max_rows > 16) return B200Q_EINVAL;
+    const int d = kv->d;
+    if (workspace_bytes < attend_ws(hq, kv->hkv, d, max_rows)) return B200Q_ENOSPACE;
     if (rows == 0) return B200Q_OK;
-    const AttnArgs a = attn_args(q, ldq, rows, hq, hkv, pages, page, {table, lens, cu, ldt, width, batch}, max_rows, scale, softcap, window,
-                                 out, ldo, workspace);
+    const AttnArgs a = attn_args(*kv, q, ldq, rows, hq, max_rows, scale, softcap, window, out, ldo, workspace);
     CUtensorMap mk, mv;
-    if (!kv_tensor_map(&mk, k_pages, k_stride, pages, page, hkv, d, kUnit, d / 64) ||
-        !kv_tensor_map(&mv, v_pages, v_stride, pages, page, hkv, d, kUnit, d / 64))
+    if (!kv_tensor_map(&mk, kv->k_pages, kv->k_stride, *kv, kUnit, d / 64) ||
+        !kv_tensor_map(&mv, kv->v_pages, kv->v_stride, *kv, kUnit, d / 64))
         return status_from(cudaErrorInvalidValue);
     const cudaStream_t s = (cudaStream_t)stream;
     const int nt = row_tiles((int64_t)max_rows * a.group);

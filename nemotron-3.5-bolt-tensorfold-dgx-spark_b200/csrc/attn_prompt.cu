@@ -555,27 +555,21 @@ size_t b200q_attn_prompt_workspace_bytes(int hq, int hkv, int d, int rows, int m
     return n == 1 ? 16 : (size_t)ctas * (sizeof(Desc) + n * (size_t)kRows * (d + 2) * sizeof(float));
 }
 
-int b200q_attn_prompt(const void* q, int64_t ldq, int rows, int hq, const void* k_pages, const void* v_pages, int64_t k_stride,
-                      int64_t v_stride, int pages, int page, int hkv, int d, const int* table, int64_t ldt, int width,
-                      const int* lens, const int* cu, int batch, int max_rows, float scale, float softcap, int window, void* out,
-                      int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!kv_args_ok(k_pages, v_pages, k_stride, v_stride, pages, page, hkv, d, table, ldt, width, lens, cu, batch) ||
-        !attn_args_ok(q, ldq, rows, hq, hkv, d, max_rows, scale, softcap, window, out, ldo) || !workspace ||
-        !aligned(workspace, 16))
-        return B200Q_EINVAL;
-    if (workspace_bytes < b200q_attn_prompt_workspace_bytes(hq, hkv, d, rows, max_rows, batch)) return B200Q_ENOSPACE;
+int b200q_attn_prompt(const b200q_paged* kv, const void* q, int64_t ldq, int rows, int hq, int max_rows, float scale, float softcap,
+                      int window, void* out, int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!attn_ok(kv, q, ldq, rows, hq, max_rows, scale, softcap, window, out, ldo, workspace)) return B200Q_EINVAL;
+    const int d = kv->d, hkv = kv->hkv;
+    if (workspace_bytes < b200q_attn_prompt_workspace_bytes(hq, hkv, d, rows, max_rows, kv->batch)) return B200Q_ENOSPACE;
     if (rows == 0) return B200Q_OK;
     PromptArgs p = {};
-    p.a = attn_args(q, ldq, rows, hq, hkv, pages, page, {table, lens, cu, ldt, width, batch}, max_rows, scale, softcap, window, out, ldo,
-                    workspace);
-    const int64_t blocks = row_blocks(p.a.group, rows, max_rows, batch);
+    p.a = attn_args(*kv, q, ldq, rows, hq, max_rows, scale, softcap, window, out, ldo, workspace);
+    const int64_t blocks = row_blocks(p.a.group, rows, max_rows, kv->batch);
     if (blocks * hkv > (1 << 28)) return B200Q_EINVAL;
     p.blocks = (int)blocks;
     p.shares = key_shares(blocks * hkv);
     CUtensorMap mk, mv;
-    const int piece = page < kTile ? page : kTile;
-    if (!kv_tensor_map(&mk, k_pages, k_stride, pages, page, hkv, d, piece, 1) ||
-        !kv_tensor_map(&mv, v_pages, v_stride, pages, page, hkv, d, piece, 1))
+    const int piece = kv->page < kTile ? kv->page : kTile;
+    if (!kv_tensor_map(&mk, kv->k_pages, kv->k_stride, *kv, piece, 1) || !kv_tensor_map(&mv, kv->v_pages, kv->v_stride, *kv, piece, 1))
         return status_from(cudaErrorInvalidValue);
     return status_from(d == 128 ? launch_prompt<128>(mk, mv, p, (cudaStream_t)stream) : launch_prompt<64>(mk, mv, p, (cudaStream_t)stream));
 }

@@ -187,26 +187,26 @@ static cudaError_t launch_append(const AppendArgs& a, int interleaved, cudaStrea
 
 using namespace b200q;
 
-extern "C" int b200q_kv_append(const void* q, const void* k, const void* v, int x_dtype, int64_t ldq, int64_t ldk, int64_t ldv,
-                               int rows, int hq, int hkv, int d, void* k_pages, void* v_pages, int64_t k_stride,
-                               int64_t v_stride, int pages, int page, const int* table, int64_t ldt, int width, const int* lens,
-                               const int* cu, int batch, const float* inv_freq, int rope, int interleaved, const void* q_norm,
-                               const void* k_norm, int norm_dtype, float eps, void* q_out, int64_t ldo, void* stream) {
-    const int e = x_dtype == B200Q_F32 ? 4 : 2;
-    if (!kv_args_ok(k_pages, v_pages, k_stride, v_stride, pages, page, hkv, d, table, ldt, width, lens, cu, batch) || rows < 0 ||
-        hq < 0 || hq > 4096 || (x_dtype != B200Q_F32 && x_dtype != B200Q_BF16) || !k || !v || (hq > 0 && (!q || !q_out)) ||
-        !aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(q_out, 16) || (ldq * e) % 16 || (ldk * e) % 16 ||
-        (ldv * e) % 16 || ldo % 8 || (hq > 0 && (ldq < (int64_t)hq * d || ldo < (int64_t)hq * d)) || ldk < (int64_t)hkv * d ||
-        ldv < (int64_t)hkv * d || rope < 0 || rope > d || rope % 16 || (rope && !inv_freq) || !aligned(inv_freq, 4) ||
+extern "C" int b200q_kv_append(const b200q_paged* kv, const void* q, const void* k, const void* v, int x_dtype, int64_t ldq,
+                               int64_t ldk, int64_t ldv, int rows, int hq, const float* inv_freq, int rope, int interleaved,
+                               const void* q_norm, const void* k_norm, int norm_dtype, float eps, void* q_out, int64_t ldo,
+                               void* stream) {
+    if (!kv_ok(kv)) return B200Q_EINVAL;
+    const int e = x_dtype == B200Q_F32 ? 4 : 2, d = kv->d;
+    const int64_t wq = (int64_t)hq * d, wk = (int64_t)kv->hkv * d;
+    if (rows < 0 || hq < 0 || hq > 4096 || (x_dtype != B200Q_F32 && x_dtype != B200Q_BF16) || !k || !v ||
+        (hq > 0 && (!q || !q_out || ldq < wq || ldo < wq)) || !aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) ||
+        !aligned(q_out, 16) || (ldq * e) % 16 || (ldk * e) % 16 || (ldv * e) % 16 || ldo % 8 || ldk < wk || ldv < wk ||
+        rope < 0 || rope > d || rope % 16 || (rope && !inv_freq) || !aligned(inv_freq, 4) ||
         ((q_norm || k_norm) && ((norm_dtype != B200Q_F32 && norm_dtype != B200Q_BF16) || !(eps >= 0.f))) ||
         !aligned(q_norm, 16) || !aligned(k_norm, 16))
         return B200Q_EINVAL;
     if (rows == 0) return B200Q_OK;
     AppendArgs a = {};
-    a.q = q; a.k = k; a.v = v; a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.rows = rows; a.hq = hq; a.hkv = hkv;
-    a.kp = (__nv_bfloat16*)k_pages; a.vp = (__nv_bfloat16*)v_pages; a.k_stride = k_stride; a.v_stride = v_stride;
-    a.pages = pages; a.page_log2 = log2_of(page);
-    a.s = {table, lens, cu, ldt, width, batch};
+    a.q = q; a.k = k; a.v = v; a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.rows = rows; a.hq = hq; a.hkv = kv->hkv;
+    a.kp = (__nv_bfloat16*)kv->k_pages; a.vp = (__nv_bfloat16*)kv->v_pages; a.k_stride = kv->k_stride; a.v_stride = kv->v_stride;
+    a.pages = kv->pages; a.page_log2 = log2_of(kv->page);
+    a.s = kv_seqs(*kv);
     a.inv_freq = inv_freq; a.rope = rope; a.q_norm = q_norm; a.k_norm = k_norm; a.norm_dtype = norm_dtype; a.eps = eps;
     a.qo = (__nv_bfloat16*)q_out; a.ldo = ldo;
     const cudaStream_t s = (cudaStream_t)stream;

@@ -21,13 +21,15 @@ inline int log2_of(int v) { int l = 0; while ((1 << l) < v) l++; return l; }
 inline bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
 
 // what every entry point asks of the cache and the step's description
-inline bool kv_args_ok(const void* k, const void* v, int64_t k_stride, int64_t v_stride, int pages, int page, int hkv, int d,
-                       const int* table, int64_t ldt, int width, const int* lens, const int* cu, int batch) {
-    return k && v && table && lens && cu && aligned(k, 16) && aligned(v, 16) && aligned(table, 4) && aligned(lens, 4) &&
-           aligned(cu, 4) && (d == 64 || d == 128) && kv_page_ok(page) && pages > 0 && hkv > 0 && hkv <= 1024 && width > 0 &&
-           ldt >= width && (int64_t)width * page <= (1 << 30) && batch > 0 && batch <= 4096 &&
-           k_stride >= (int64_t)hkv * page * d && v_stride >= (int64_t)hkv * page * d && k_stride % 8 == 0 && v_stride % 8 == 0 &&
-           k_stride < ((int64_t)1 << 38) && v_stride < ((int64_t)1 << 38);
+inline bool kv_ok(const b200q_paged* p) {
+    if (!p) return false;
+    const int64_t one = (int64_t)p->hkv * p->page * p->d, far = (int64_t)1 << 38;
+    return p->k_pages && p->v_pages && p->table && p->lens && p->cu && aligned(p->k_pages, 16) && aligned(p->v_pages, 16) &&
+           aligned(p->table, 4) && aligned(p->lens, 4) && aligned(p->cu, 4) && (p->d == 64 || p->d == 128) && kv_page_ok(p->page) &&
+           p->pages > 0 && p->hkv > 0 && p->hkv <= 1024 && p->width > 0 && p->ldt >= p->width &&
+           (int64_t)p->width * p->page <= (1 << 30) && p->batch > 0 && p->batch <= 4096 && p->k_stride >= one &&
+           p->v_stride >= one && p->k_stride % 8 == 0 && p->v_stride % 8 == 0 && p->k_stride < far && p->v_stride < far;
 }
+inline KvSeqs kv_seqs(const b200q_paged& p) { return {p.table, p.lens, p.cu, p.ldt, p.width, p.batch}; }
 
 }  // namespace b200q

@@ -1,6 +1,5 @@
 """CPU tests of the paged attention operators: every refusal comes before a launch (the addresses below are never read),
 and the fp64 definitions the GPU tests use are themselves checked."""
-import ctypes
 import math
 
 import pytest
@@ -9,64 +8,64 @@ import torch
 import b200q
 from paged import Step, attend, rotate
 
-vp = ctypes.c_void_p
 A = 0x100000   # aligned addresses that nothing reads
 
 
-def append_args(**kw):
-    a = dict(q=vp(A), k=vp(A), v=vp(A), x_dtype=0, ldq=512, ldk=256, ldv=256, rows=4, hq=4, hkv=2, d=128, kp=vp(A), vp_=vp(A),
-             ks=2 * 16 * 128, vs=2 * 16 * 128, pages=8, page=16, table=vp(A), ldt=4, width=4, lens=vp(A), cu=vp(A), batch=2,
-             inv=vp(A), rope=64, inter=0, qn=None, kn=None, nd=0, eps=1e-6, qo=vp(A), ldo=512, stream=None)
-    assert set(kw) <= set(a)
-    a.update(kw)
-    return list(a.values())
+CACHE = dict(kp=A, vp=A, ks=2 * 16 * 128, vs=2 * 16 * 128, table=A, lens=A, cu=A, ldt=4, pages=8, page=16, hkv=2, d=128, width=4,
+             batch=2)
+APPEND = dict(q=A, k=A, v=A, x_dtype=0, ldq=512, ldk=256, ldv=256, rows=4, hq=4, inv=A, rope=64, inter=0, qn=0, kn=0, nd=0,
+              eps=1e-6, qo=A, ldo=512, stream=0)
+ATTN = dict(q=A, ldq=512, rows=4, hq=4, max_rows=4, scale=0.1, softcap=0.0, window=0, out=A, ldo=512, ws=A, wsb=1 << 40, stream=0)
 
 
-CACHE_REFUSALS = [dict(kp=None), dict(vp_=None), dict(kp=vp(A + 8)), dict(ks=2 * 16 * 128 - 8), dict(vs=2 * 16 * 128 + 4),
-                  dict(pages=0), dict(page=8), dict(page=48), dict(page=512), dict(d=96), dict(hkv=0), dict(table=None),
-                  dict(width=5), dict(width=0), dict(lens=None), dict(cu=None), dict(cu=vp(A + 2)), dict(batch=0),
-                  dict(batch=4097), dict(width=1 << 27, ldt=1 << 27)]
+def call(name, base, kw):
+    """the C entry point with a good call's arguments but for those in kw"""
+    assert set(kw) <= set(CACHE) | set(base)
+    kv = b200q._PAGED.pack(*(kw.get(n, x) for n, x in CACHE.items()))
+    return getattr(b200q.lib(), name)(kv, *(kw.get(n, x) for n, x in base.items()))
+
+
+def append(**kw):
+    return call("b200q_kv_append", APPEND, kw)
+
+
+CACHE_REFUSALS = [dict(kp=0), dict(vp=0), dict(kp=A + 8), dict(ks=2 * 16 * 128 - 8), dict(vs=2 * 16 * 128 + 4), dict(ks=1 << 39),
+                  dict(pages=0), dict(page=8), dict(page=48), dict(page=512), dict(d=96), dict(hkv=0), dict(hkv=-2), dict(table=0),
+                  dict(width=5), dict(width=0), dict(lens=0), dict(cu=0), dict(cu=A + 2), dict(batch=0), dict(batch=4097),
+                  dict(width=1 << 27, ldt=1 << 27)]
 
 
 @pytest.mark.parametrize("kw", CACHE_REFUSALS + [
-    dict(k=None), dict(v=None), dict(q=None), dict(qo=None), dict(q=vp(A + 4)), dict(x_dtype=2), dict(ldq=511), dict(ldq=508),
-    dict(ldk=128), dict(ldv=130), dict(ldo=504), dict(rope=8), dict(rope=144), dict(rope=-16), dict(inv=None), dict(rows=-1),
-    dict(hq=-1), dict(hq=5000), dict(qn=vp(A), nd=3), dict(qn=vp(A + 8)), dict(kn=vp(A), eps=-1.0),
-    dict(kn=vp(A), eps=float("nan"))])
+    dict(k=0), dict(v=0), dict(q=0), dict(qo=0), dict(q=A + 4), dict(x_dtype=2), dict(ldq=511), dict(ldq=508), dict(ldk=128),
+    dict(ldv=130), dict(ldo=504), dict(rope=8), dict(rope=144), dict(rope=-16), dict(inv=0), dict(rows=-1), dict(hq=-1),
+    dict(hq=5000), dict(qn=A, nd=3), dict(qn=A + 8), dict(kn=A, eps=-1.0), dict(kn=A, eps=float("nan"))])
 def test_append_refuses(kw):
-    assert b200q.lib().b200q_kv_append(*append_args(**kw)) == b200q.EINVAL
+    assert append(**kw) == b200q.EINVAL
 
 
 def test_append_of_no_rows_is_nothing():
-    assert b200q.lib().b200q_kv_append(*append_args(rows=0)) == b200q.OK
-
-
-def attn_args(**kw):
-    a = dict(q=vp(A), ldq=512, rows=4, hq=4, kp=vp(A), vp_=vp(A), ks=2 * 16 * 128, vs=2 * 16 * 128, pages=8, page=16, hkv=2, d=128,
-             table=vp(A), ldt=4, width=4, lens=vp(A), cu=vp(A), batch=2, max_rows=4, scale=0.1, softcap=0.0, window=0, out=vp(A),
-             ldo=512, ws=vp(A), wsb=1 << 40, stream=None)
-    assert set(kw) <= set(a)
-    a.update(kw)
-    return list(a.values())
+    assert append(rows=0) == b200q.OK
+    assert b200q.lib().b200q_kv_append(None, *APPEND.values()) == b200q.EINVAL
 
 
 @pytest.mark.parametrize("f", ["b200q_attn_decode", "b200q_attn_prompt"])
 @pytest.mark.parametrize("kw", CACHE_REFUSALS + [
-    dict(q=None), dict(out=None), dict(q=vp(A + 8)), dict(out=vp(A + 4)), dict(ldq=504), dict(ldo=516), dict(rows=-1), dict(hq=0),
-    dict(hq=5), dict(max_rows=0), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
-    dict(softcap=-1.0), dict(softcap=float("nan")), dict(window=-1), dict(ws=None), dict(ws=vp(A + 8))])
+    dict(q=0), dict(out=0), dict(q=A + 8), dict(out=A + 4), dict(ldq=504), dict(ldo=516), dict(rows=-1), dict(hq=0), dict(hq=5),
+    dict(max_rows=0), dict(max_rows=1 << 30), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
+    dict(scale=float("inf")), dict(softcap=-1.0), dict(softcap=float("nan")), dict(window=-1), dict(ws=0), dict(ws=A + 8)])
 def test_attention_refuses(f, kw):
-    assert getattr(b200q.lib(), f)(*attn_args(**kw)) == b200q.EINVAL
+    assert call(f, ATTN, kw) == b200q.EINVAL
 
 
 def test_attention_of_no_rows_too_many_and_too_little_workspace():
     L = b200q.lib()
-    for f in (L.b200q_attn_decode, L.b200q_attn_prompt):
-        assert f(*attn_args(rows=0)) == b200q.OK
-        assert f(*attn_args(wsb=16)) == b200q.ENOSPACE
-    assert L.b200q_attn_decode(*attn_args(max_rows=17)) == b200q.EINVAL
+    for f in ("b200q_attn_decode", "b200q_attn_prompt"):
+        assert call(f, ATTN, dict(rows=0)) == b200q.OK
+        assert call(f, ATTN, dict(wsb=0)) == b200q.ENOSPACE
+    assert call("b200q_attn_decode", ATTN, dict(max_rows=17)) == b200q.EINVAL
     assert L.b200q_attn_decode_workspace_bytes(4, 2, 128, 17) == 0
     assert 0 < L.b200q_attn_decode_workspace_bytes(32, 8, 128, 1) <= 8 << 20
+    assert 0 < L.b200q_attn_prompt_workspace_bytes(32, 8, 128, 77, 77, 1) <= 64 << 20
 
 
 def test_host_tensors_are_refused():
