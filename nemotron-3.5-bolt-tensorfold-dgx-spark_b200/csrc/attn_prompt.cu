@@ -45,7 +45,7 @@ template <int D>
 struct Lay {
     static constexpr int kBytes = kTile * D * 2;              // a tile of Q, K or V: [D / 64][128][128 B]
     static constexpr int kStages = D == 128 ? 2 : 4;          // of K and of V
-    static constexpr int kBars = 4 * kStages + 9;
+    static constexpr int kBars = 4 * kStages + 11;
     static constexpr size_t kSlot = (size_t)kRows * (D + 2);  // floats of a partial: O [256][D], m [256], sum [256]
     static size_t smem(int batch) { return 1024 + (2 + 2 * kStages) * (size_t)kBytes + kBars * 8 + 16 + (size_t)(batch + 1) * 4; }
 };
@@ -87,10 +87,62 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
           "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
           "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *(uint32_t*)&v;
+}
+// one lane of a converged warp, as the compiler knows: MMA operands then stay in uniform registers
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(p));
+    return p != 0;
+}
+// two fp32 at a time
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {   // NaN if any is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^x for two x <= 8, without the special-function unit: x = n + f, |f| <= 1/2, and 2^f by the polynomial of degree 3
+// with the least relative error there (7.5e-5 = 2^-13.7, a Remez fit; the result is rounded to bf16 next, 2^-8).  Below
+// 2^-126 it stays there.  Adding 1.5 2^23 leaves n in the low bits of the sum, and n << 23 adds to the exponent.
+__device__ __forceinline__ void ex2_poly(uint64_t x, float& lo, float& hi) {
+    const uint64_t magic = pair(12582912.f, 12582912.f);
+    float a, b;
+    unpair(x, a, b);
+    x = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
+    const uint64_t t = add2(x, magic), n = add2(t, pair(-12582912.f, -12582912.f)), f = fma2(n, pair(-1.f, -1.f), x);
+    uint64_t p = fma2(pair(0.05517166852951050f, 0.05517166852951050f), f, pair(0.24261112511157990f, 0.24261112511157990f));
+    p = fma2(p, f, pair(0.69326096773147583f, 0.69326096773147583f));
+    p = fma2(p, f, pair(0.99992805719375610f, 0.99992805719375610f));
+    float n0, n1;
+    unpair(t, n0, n1);
+    unpair(p, a, b);
+    lo = __uint_as_float(__float_as_uint(a) + (__float_as_uint(n0) << 23));
+    hi = __uint_as_float(__float_as_uint(b) + (__float_as_uint(n1) << 23));
 }
 // rows row .. of one 64-value column block `chunk` of page `page`, kv head `head`
 __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* m, int row, int chunk, int head, int page, uint32_t bar) {
@@ -117,7 +169,7 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
     uint8_t* base = smem_raw + (sq - raw);
     const uint32_t sk = sq + 2 * L::kBytes, sv = sk + NS * L::kBytes, bars = sv + NS * L::kBytes;
     const uint32_t kfull = bars, kempty = kfull + NS * 8, vfull = kempty + NS * 8, vempty = vfull + NS * 8;
-    const uint32_t qfull = vempty + NS * 8, sfull = qfull + 8, pready = sfull + 16, odone = pready + 16;   // odone [2], last
+    const uint32_t qfull = vempty + NS * 8, sfull = qfull + 8, pready = sfull + 16, odone = pready + 32;   // odone [2], last
     const uint32_t tslot = bars + L::kBars * 8;
     int* pre = (int*)(base + (tslot + 16 - sq));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -214,7 +266,8 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
         tc_mbar_init(qfull, 256);
         for (int t = 0; t < 2; t++) {
             tc_mbar_init(sfull + t * 8, 1);
-            tc_mbar_init(pready + t * 8, 128);
+            tc_mbar_init(pready + t * 16, 128);
+            tc_mbar_init(pready + t * 16 + 8, 128);
             tc_mbar_init(odone + t * 8, 1);
         }
         tc_mbar_init(odone + 16, 1);
@@ -275,12 +328,12 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
             bool dead = !tc_mbar_wait(qfull, 0);
             int pr[2] = {0, 0};   // P tiles used so far
             auto scores = [&](int t, int st) {
-                if (lane == 0) {
+                const uint64_t qd = umma_desc_sw128(sq + t * L::kBytes), kd = umma_desc_sw128(sk + st * L::kBytes);
+                if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < D / 16; k++) {
-                        const uint32_t off = (k / 4) * (kTile * 128) + (k % 4) * 32;
-                        umma_ss(tmem + t * kTile, umma_desc_sw128(sq + t * L::kBytes + off), umma_desc_sw128(sk + st * L::kBytes + off),
-                                kIdescQK, k > 0);
+                        const uint32_t off = ((k / 4) * (kTile * 128) + (k % 4) * 32) >> 4;
+                        umma_ss(tmem + t * kTile, qd + off, kd + off, kIdescQK, k > 0);
                     }
                     umma_commit(sfull + t * 8);
                 }
@@ -293,7 +346,7 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                     tc_fence_after();
                     for (int t = 0; t < 2; t++)
                         if (ja[t] == j0 && jb[t] > j0) scores(t, 0);
-                    if (lane == 0) umma_commit(kempty);
+                    if (elect_one()) umma_commit(kempty);
                 }
             }
             for (int j = j0; j < j1 && !dead; j++) {
@@ -314,30 +367,35 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                 }
                 for (int t = 0; t < 2; t++) {
                     if (j >= ja[t] && j < jb[t]) {
-                        if (!tc_mbar_wait(pready + t * 8, pr[t] & 1)) dead = true;
-                        dead = __any_sync(~0u, dead);
-                        if (dead) break;
-                        tc_fence_after();
-                        if (lane == 0) {
 #pragma unroll
-                            for (int k = 0; k < kTile / 16; k++)
-                                umma_ts(tmem + 256 + t * D, tmem + t * kTile + k * 8, desc_v(sv + st * L::kBytes + k * 2048), kIdescPV<D>,
-                                        pr[t] > 0 || k > 0);
-                            umma_commit(odone + t * 8);
+                        for (int half = 0; half < 2; half++) {
+                            if (!tc_mbar_wait(pready + (t * 2 + half) * 8, pr[t] & 1)) dead = true;
+                            dead = __any_sync(~0u, dead);
+                            if (dead) break;
+                            tc_fence_after();
+                            const uint64_t vd = desc_v(sv + st * L::kBytes);
+                            if (elect_one()) {
+#pragma unroll
+                                for (int k = half * 4; k < half * 4 + 4; k++)
+                                    umma_ts(tmem + 256 + t * D, tmem + t * kTile + k * 8, vd + k * (2048 >> 4), kIdescPV<D>,
+                                            pr[t] > 0 || k > 0);
+                            }
                         }
+                        if (dead) break;
+                        if (elect_one()) umma_commit(odone + t * 8);
                         __syncwarp();
                         pr[t]++;
                     }
                     if (j + 1 >= ja[t] && j + 1 < jb[t]) scores(t, sn);
                 }
                 if (dead) break;
-                if (lane == 0) {
+                if (elect_one()) {
                     umma_commit(vempty + st * 8);
                     if (j + 1 < j1) umma_commit(kempty + sn * 8);
                 }
                 __syncwarp();
             }
-            if (lane == 0) umma_commit(odone + 16);   // every MMA issued
+            if (elect_one()) umma_commit(odone + 16);   // every MMA issued
             __syncwarp();
             tc_mbar_wait(odone + 16, 0);
             if (dead && lane == 0) atomicOr(&g_prompt_error, 1);
@@ -374,21 +432,29 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
 #pragma unroll
             for (int k = 0; k < 4; k++) tmem_ld32(ts + k * 32, s[k]);
             tmem_ld_wait();
-            float top = -INFINITY;
             if (a.cap_in != 0.f)
 #pragma unroll
                 for (int k = 0; k < kTile; k++) s[k / 32][k % 32] = __float_as_uint(capped(__uint_as_float(s[k / 32][k % 32]), a.cap_in));
-            if (key0 + kTile - 1 > p0[t] || key0 <= p1[t] - a.window) {   // some row does not see some key
+            bool exact = key0 + kTile - 1 > p0[t] || key0 <= p1[t] - a.window;   // some row does not see some key
+            if (exact) {
                 const int last = pos - key0, first = pos - a.window - key0;
 #pragma unroll
                 for (int k = 0; k < kTile; k++)
                     if (k > last || k <= first) s[k / 32][k % 32] = 0xff800000u;
             }
+            float tops[4];
 #pragma unroll
-            for (int k = 0; k < kTile; k++) top = fmaxf(top, __uint_as_float(s[k / 32][k % 32]));
-            top *= c;
-            if (__any_sync(~0u, top > ref + 8.f)) {
-                const float now = top > ref + 8.f ? top : ref, f = ex2(ref - (now == -INFINITY ? 0.f : now));
+            for (int k = 0; k < 4; k++) tops[k] = max3(__uint_as_float(s[k][0]), __uint_as_float(s[k][1]), __uint_as_float(s[k][2]));
+#pragma unroll
+            for (int x = 3; x < 31; x += 2)
+#pragma unroll
+                for (int k = 0; k < 4; k++) tops[k] = max3(tops[k], __uint_as_float(s[k][x]), __uint_as_float(s[k][x + 1]));
+#pragma unroll
+            for (int k = 0; k < 4; k++) tops[k] = max3(tops[k], tops[k], __uint_as_float(s[k][31]));
+            const float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]) * c;
+            if (__any_sync(~0u, !(top <= ref + 8.f))) {
+                // an infinite or NaN score makes its row NaN: by the reference, since ex2_poly does not carry NaN
+                const float now = top <= ref + 8.f ? ref : top < INFINITY ? top : NAN, f = ex2(ref - (now == -INFINITY ? 0.f : now));
                 ref = now;
                 sum *= f;
                 if (i > 0) {
@@ -406,22 +472,38 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                     }
                 }
             }
+            exact |= __any_sync(~0u, ref == -INFINITY);
             const float z = ref == -INFINITY ? 0.f : ref;
+            const uint64_t c2 = pair(c, c), z2 = pair(-z, -z);
+            uint64_t sum2 = pair(0.f, 0.f);
+            auto exps = [&](bool all) {
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                uint32_t p[32];
+                for (int k = 0; k < 4; k++) {
+                    uint32_t p[16];
 #pragma unroll
-                for (int x = 0; x < 32; x++) {
-                    const float e0 = ex2(fmaf(__uint_as_float(s[2 * k + x / 16][x % 16 * 2]), c, -z));
-                    const float e1 = ex2(fmaf(__uint_as_float(s[2 * k + x / 16][x % 16 * 2 + 1]), c, -z));
-                    sum += e0 + e1;
-                    p[x] = pack2(e0, e1);
+                    for (int x = 0; x < 16; x++) {
+                        const uint64_t e = fma2(pair(__uint_as_float(s[k][2 * x]), __uint_as_float(s[k][2 * x + 1])), c2, z2);
+                        float e0, e1;
+                        if (all || x % 4 != 3) {
+                            unpair(e, e0, e1);
+                            e0 = ex2(e0);
+                            e1 = ex2(e1);
+                        } else ex2_poly(e, e0, e1);
+                        sum2 = add2(sum2, pair(e0, e1));
+                        p[x] = pack2(e0, e1);
+                    }
+                    tmem_st16(ts + k * 16, p);
+                    if (k & 1) {   // half of P: its product may begin
+                        tmem_st_wait();
+                        tc_fence_before();
+                        tc_mbar_arrive(pready + (t * 2 + k / 2) * 8);
+                    }
                 }
-                tmem_st32(ts + k * 32, p);
-            }
-            tmem_st_wait();
-            tc_fence_before();
-            tc_mbar_arrive(pready + t * 8);
+            };
+            if (exact) exps(true); else exps(false);
+            float s0, s1;
+            unpair(sum2, s0, s1);
+            sum += s0 + s1;
         }
         // ---------------------------------------------------------------- out
         if (n > 0 && !dead && !tc_mbar_wait(odone + t * 8, (n - 1) & 1)) dead = true;
