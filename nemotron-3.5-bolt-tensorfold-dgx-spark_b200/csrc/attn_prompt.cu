@@ -40,6 +40,10 @@ constexpr int kRows = 2 * kTile;      // rows of a CTA
 constexpr int kThreads = 384;         // two softmax warpgroups; MMA and TMA warps
 constexpr int kMinSteps = 4;          // a share of a cut row block has at least so many steps of keys
 constexpr int kMaxShares = 32;
+#ifndef KPOLY
+#define KPOLY 2
+#endif
+constexpr int kPoly = KPOLY;              // of 8 pairs of exponentials, those by polynomial
 
 template <int D>
 struct Lay {
@@ -352,7 +356,6 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
             for (int j = j0; j < j1 && !dead; j++) {
                 const int n = j - j0, st = n % NS, sn = (n + 1) % NS;
                 if (!tc_mbar_wait(vfull + st * 8, n / NS & 1)) dead = true;
-                if (j + 1 < j1 && !tc_mbar_wait(kfull + sn * 8, (n + 1) / NS & 1)) dead = true;
                 dead = __any_sync(~0u, dead);
                 if (dead) break;
                 const int key0 = j * kTile;
@@ -386,13 +389,16 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                         __syncwarp();
                         pr[t]++;
                     }
+                    if (t == 1 && elect_one()) umma_commit(vempty + st * 8);
+                    if (t == 0 && j + 1 < j1) {
+                        if (!tc_mbar_wait(kfull + sn * 8, (n + 1) / NS & 1)) dead = true;
+                        dead = __any_sync(~0u, dead);
+                        if (dead) break;
+                    }
                     if (j + 1 >= ja[t] && j + 1 < jb[t]) scores(t, sn);
                 }
                 if (dead) break;
-                if (elect_one()) {
-                    umma_commit(vempty + st * 8);
-                    if (j + 1 < j1) umma_commit(kempty + sn * 8);
-                }
+                if (j + 1 < j1 && elect_one()) umma_commit(kempty + sn * 8);
                 __syncwarp();
             }
             if (elect_one()) umma_commit(odone + 16);   // every MMA issued
@@ -475,7 +481,7 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
             exact |= __any_sync(~0u, ref == -INFINITY);
             const float z = ref == -INFINITY ? 0.f : ref;
             const uint64_t c2 = pair(c, c), z2 = pair(-z, -z);
-            uint64_t sum2 = pair(0.f, 0.f);
+            uint64_t sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
             auto exps = [&](bool all) {
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -484,12 +490,12 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                     for (int x = 0; x < 16; x++) {
                         const uint64_t e = fma2(pair(__uint_as_float(s[k][2 * x]), __uint_as_float(s[k][2 * x + 1])), c2, z2);
                         float e0, e1;
-                        if (all || x % 4 != 3) {
+                        if (all || x * kPoly % 8 < 8 - kPoly) {
                             unpair(e, e0, e1);
                             e0 = ex2(e0);
                             e1 = ex2(e1);
                         } else ex2_poly(e, e0, e1);
-                        sum2 = add2(sum2, pair(e0, e1));
+                        sums[x & 1] = add2(sums[x & 1], pair(e0, e1));
                         p[x] = pack2(e0, e1);
                     }
                     tmem_st16(ts + k * 16, p);
@@ -502,7 +508,7 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
             };
             if (exact) exps(true); else exps(false);
             float s0, s1;
-            unpair(sum2, s0, s1);
+            unpair(add2(sums[0], sums[1]), s0, s1);
             sum += s0 + s1;
         }
         // ---------------------------------------------------------------- out
