@@ -47,7 +47,6 @@ __device__ __forceinline__ void tma_kv(uint32_t dst, const CUtensorMap* m, int r
 
 // the tensor map of one side of the cache: dims (64, page, d / 64, heads, pages), box (64, box_rows, box_blocks, 1, 1)
 bool kv_tensor_map(CUtensorMap* m, const void* pages, int64_t stride, const b200q_paged& kv, int box_rows, int box_blocks);
-int attn_sms();   // SMs of the current device
 
 // the checks both forms share
 inline bool attn_ok(const b200q_paged* kv, const void* q, int64_t ldq, int rows, int hq, int max_rows, float scale, float softcap,

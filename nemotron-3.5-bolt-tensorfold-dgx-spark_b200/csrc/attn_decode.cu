@@ -33,19 +33,6 @@ int attn_error_read(int clear) {
     return v;
 }
 
-int attn_sms() {
-    static int sms[64] = {0};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) dev = 0;
-    if (!sms[dev]) {
-        int v = 0;
-        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
-        sms[dev] = v > 0 ? v : 148;
-    }
-    return sms[dev];
-}
-
 bool kv_tensor_map(CUtensorMap* m, const void* pages, int64_t stride, const b200q_paged& kv, int box_rows, int box_blocks) {
     typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -566,7 +553,7 @@ cudaError_t launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const Attn
     const size_t smem = Shape<D, NT>::smem(a.s.batch);
     cudaError_t e = cudaFuncSetAttribute(attn_rows_k<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    const int ctas = min(attn_sms(), kMaxCtas);
+    const int ctas = min(device_sms(), kMaxCtas);
     e = launch(attn_rows_k<D, NT>, dim3(ctas), dim3((kWarps + 1) * 32), smem, s, mk, mv, a);
     if (e != cudaSuccess) return e;
     return launch(attn_join_k<D, NT>, dim3(ctas), dim3(256), 0, s, a);

@@ -40,10 +40,7 @@ constexpr int kRows = 2 * kTile;      // rows of a CTA
 constexpr int kThreads = 384;         // two softmax warpgroups; MMA and TMA warps
 constexpr int kMinSteps = 4;          // a share of a cut row block has at least so many steps of keys
 constexpr int kMaxShares = 32;
-#ifndef KPOLY
-#define KPOLY 2
-#endif
-constexpr int kPoly = KPOLY;              // of 8 pairs of exponentials, those by polynomial
+constexpr int kPoly = 2;              // of 8 pairs of exponentials, those by polynomial
 
 template <int D>
 struct Lay {
@@ -615,7 +612,7 @@ int64_t row_blocks(int group, int rows, int max_rows, int batch) {
     return by_rows < by_seq ? by_rows : by_seq;
 }
 int key_shares(int64_t ctas) {
-    const int64_t n = attn_sms() / (ctas > 0 ? ctas : 1);
+    const int64_t n = device_sms() / (ctas > 0 ? ctas : 1);
     return n < 1 ? 1 : n > kMaxShares ? kMaxShares : (int)n;
 }
 

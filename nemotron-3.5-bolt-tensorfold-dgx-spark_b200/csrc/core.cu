@@ -16,6 +16,19 @@ bool pdl_enabled() {
     return on;
 }
 
+int device_sms() {
+    static int sms[64] = {0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) dev = 0;
+    if (!sms[dev]) {
+        int v = 0;
+        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
+        sms[dev] = v > 0 ? v : 148;
+    }
+    return sms[dev];
+}
+
 // the error words of the sources that keep one, weak: a library built without the IQ2_XXS tables leaves two of them out
 __attribute__((weak)) int iq2_error_read(int clear);    // iq2.cu
 __attribute__((weak)) int tc_error_read(int clear);     // tc_gemm.cu

@@ -7,11 +7,13 @@
 //
 // The angle is a product of a position and an fp32 frequency, formed and reduced by 2 pi in fp64 (exact but for the
 // reduction's last bits: at position 2^18 an fp32 angle would be off by up to 2^-7), then one sincosf of the remainder.
-// cos and sin depend on the token alone, so a CTA computes them once for all heads of its token, in shared memory.
+// cos and sin depend on the token alone: a warp computes its row's once for all heads it takes.
 //
-// Bound by HBM: every input value is read once and every output written once (bf16).  A CTA takes one token; each of its
-// warps keeps kUnroll loads of 32 lanes x 8 values in flight before the first is used (a head is d / 8 lanes, so a warp's
-// load covers two heads of 128 or four of 64, and the partner of a rotated half is a shuffle away).
+// Bound by HBM: every input value is read once and every output written once (bf16).  A warp takes some of a row's
+// heads, two of 128 or four of 64 a load; its first batch of loads leaves before the row's place in the cache is known
+// (a chain of loads of cu, lens, table), and a pair to rotate lies in one lane, so rows cost few instructions besides.
+// Measured: 8192 fp32 rows of 48 heads of 128 (norm, half rotated; 302 MB) 57.8 us = 5.2 TB/s, 80 % of the measured
+// copy rate; 5560 bf16 rows of 72 heads of 64 (102 MB) 23.6 us = 4.3 TB/s; one row 2.7 us.
 #include "kv.cuh"
 
 namespace b200q {
@@ -46,24 +48,29 @@ struct AppendArgs {
 };
 
 constexpr int kAppendWarps = 8;
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]);
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
-    const float4 a = *(const float4*)p, b = *((const float4*)p + 1);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+// Four values as they lie in memory, and kept so while in flight; loads a batch (what 64 registers hold, four CTAs an
+// SM: three CTAs, or five with spills, were 10 to 60 % slower), loads a warp (its row's place and angles are found once)
+template <typename T> struct Raw;
+template <> struct Raw<float> {
+    typedef float4 type;
+    static constexpr int kUnroll = 3, kLoads = 12;
+};
+template <> struct Raw<__nv_bfloat16> {
+    typedef uint2 type;
+    static constexpr int kUnroll = 5, kLoads = 10;
+};
+__device__ __forceinline__ void widen(float4 v, float* x) { x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
+__device__ __forceinline__ void widen(uint2 v, float* x) {
+    x[0] = __uint_as_float(v.x << 16);
+    x[1] = __uint_as_float(v.x & 0xffff0000u);
+    x[2] = __uint_as_float(v.y << 16);
+    x[3] = __uint_as_float(v.y & 0xffff0000u);
 }
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[8]) {
-    const uint4 a = *(const uint4*)p;
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+template <typename T>
+__device__ __forceinline__ typename Raw<T>::type raw4(const T* p) { return *(const typename Raw<T>::type*)p; }
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float* x) {
+    __nv_bfloat162 o[2] = {__floats2bfloat162_rn(x[0], x[1]), __floats2bfloat162_rn(x[2], x[3])};   // the cache's type
+    *(uint2*)p = *(uint2*)o;
 }
 
 // the sequence that row t belongs to (batch if none), by the whole warp: the count of range ends at or before t
@@ -73,99 +80,108 @@ __device__ __forceinline__ int row_sequence(const KvSeqs& s, int t, int lane) {
     return b;
 }
 
-template <typename T, int D, bool INTERLEAVED, int U>
-__global__ void __launch_bounds__(kAppendWarps * 32) kv_append_k(AppendArgs a) {
+template <typename T, int D, bool INTERLEAVED>
+__global__ void __launch_bounds__(kAppendWarps * 32, 4) kv_append_k(AppendArgs a, int parts) {
     pdl_wait();
-    constexpr int kLanes = D / 8, kHeads = 32 / kLanes;   // lanes of a head, heads of a warp's load
-    __shared__ float2 cs[D / 2];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = blockIdx.x;
-    const int heads = a.hq + 2 * a.hkv;
-    const int sub = lane / kLanes, e0 = (lane % kLanes) * 8;   // this lane's head of the load, first value in it
+    constexpr int kLanes = D / 8, kHeads = 32 / kLanes, U = Raw<T>::kUnroll;   // lanes of a head, heads of a load
+    __shared__ float2 angles[kAppendWarps][D / 2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t task = (int64_t)blockIdx.x * kAppendWarps + warp;
+    const int t = (int)(task / parts), part = (int)(task - (int64_t)t * parts);
+    if (t >= a.rows) { pdl_trigger(); return; }
+    // This lane's eight values of a head: in the rotated part four and their four partners, so that a pair never leaves
+    // its lane, elsewhere (and where pairs stand side by side) eight in a row.
+    const int sub = lane / kLanes, hl = lane % kLanes, half = a.rope >> 1;
+    const bool turned = hl < a.rope / 8;
+    const int ea = !INTERLEAVED && turned ? 4 * hl : 8 * hl, eb = !INTERLEAVED && turned ? half + 4 * hl : 8 * hl + 4;
+    // loads: kHeads heads of q, of k or of v each
+    const int lq = (a.hq + kHeads - 1) / kHeads, lk = (a.hkv + kHeads - 1) / kHeads, loads = lq + 2 * lk;
+    auto head = [&](int l) { return (l < lq ? l : l < lq + lk ? l - lq : l - lq - lk) * kHeads + sub; };
+    typename Raw<T>::type x[U][2];
+    auto load = [&](int l0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int l = l0 + u * parts, h = head(l);
+            if (l >= loads || h >= (l < lq ? a.hq : a.hkv)) continue;
+            const T* p = (l < lq ? (const T*)a.q + t * a.ldq : l < lq + lk ? (const T*)a.k + t * a.ldk : (const T*)a.v + t * a.ldv) + h * D;
+            x[u][0] = raw4(p + ea);
+            x[u][1] = raw4(p + eb);
+        }
+    };
+    load(part);   // before the row's place is known: that is a chain of four more loads (cu, lens, table, angles)
+    float freq[D / 64];
+#pragma unroll
+    for (int i = 0; i < D / 64; i++) freq[i] = lane + 32 * i < half ? a.inv_freq[lane + 32 * i] : 0.f;
 
     const int b = row_sequence(a.s, t, lane);
     if (b >= a.s.batch || t < a.s.cu[0]) { pdl_trigger(); return; }   // padding rows
     const int pos = a.s.lens[b] - a.s.cu[b + 1] + t;
     if (pos < 0) { pdl_trigger(); return; }   // more rows than tokens: no place
     const int entry = pos >> a.page_log2;
-    int page = -1;
-    if (entry < a.s.width) page = a.s.table[b * a.s.ldt + entry];
+    const int page = entry < a.s.width ? a.s.table[b * a.s.ldt + entry] : -1;
     const bool stored = page >= 0 && page < a.pages;
-    if (!stored && threadIdx.x == 0) atomicOr(&g_kv_error, 1);
-    const int half = a.rope >> 1;
-    for (int i = threadIdx.x; i < half; i += blockDim.x) {
-        const double turn = (double)pos * (double)a.inv_freq[i];
-        const float r = (float)fma(-6.283185307179586476925, rint(turn * 0.15915494309189533577), turn);
-        float2 v;
-        sincosf(r, &v.y, &v.x);
-        cs[i] = v;
-    }
-    __syncthreads();
-
-    const int step = (int)gridDim.y * kAppendWarps * kHeads;
-    for (int h0 = ((int)blockIdx.y * kAppendWarps + warp) * kHeads; h0 < heads; h0 += step * U) {
-        float x[U][8];
+    if (!stored && part == 0 && lane == 0) atomicOr(&g_kv_error, 1);
+    const int64_t slot = (int64_t)(pos & ((1 << a.page_log2) - 1)) * D;
+    float4 c0, c1;   // (cos, sin) of this lane's four angles
+    if (half) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int h = h0 + u * step + sub;
-            if (h >= heads) continue;
-            const T* p = h < a.hq ? (const T*)a.q + t * a.ldq + h * D
-                       : h < a.hq + a.hkv ? (const T*)a.k + t * a.ldk + (h - a.hq) * D
-                                          : (const T*)a.v + t * a.ldv + (h - a.hq - a.hkv) * D;
-            load8(p + e0, x[u]);
+        for (int i = 0; i < D / 64; i++) {
+            if (lane + 32 * i >= half) break;
+            const double turn = (double)pos * (double)freq[i];
+            const float r = (float)fma(-6.283185307179586476925, rint(turn * 0.15915494309189533577), turn);
+            float2 v;
+            sincosf(r, &v.y, &v.x);
+            angles[warp][lane + 32 * i] = v;
         }
+        __syncwarp();
+        if (turned) {
+            c0 = *(const float4*)&angles[warp][4 * hl];
+            c1 = *(const float4*)&angles[warp][4 * hl + 2];
+        }
+    }
+
+    for (int l0 = part; l0 < loads; l0 += parts * U) {
+        if (l0 != part) load(l0);
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int h = h0 + u * step + sub;
-            const bool live = h < heads, is_q = h < a.hq, is_v = h >= a.hq + a.hkv;
-            const void* w = is_q ? a.q_norm : a.k_norm;
-            float ss = 0.f;
+            const int l = l0 + u * parts;
+            if (l >= loads) break;
+            const int h = head(l);
+            const bool is_q = l < lq, is_v = l >= lq + lk, live = h < (is_q ? a.hq : a.hkv);
+            float y[8];
+            widen(x[u][0], y);
+            widen(x[u][1], y + 4);
+            if (!is_v) {
+                const void* w = is_q ? a.q_norm : a.k_norm;
+                if (w) {
+                    float ss = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; j++) ss = fmaf(x[u][j], x[u][j], ss);
+                    for (int j = 0; j < 8; j++) ss = fmaf(y[j], y[j], ss);
 #pragma unroll
-            for (int m = kLanes / 2; m; m >>= 1) ss += __shfl_xor_sync(~0u, ss, m);
-            if (live && !is_v && w) {
-                const float r = rsqrtf(ss * (1.f / D) + a.eps);
-                float wv[8];
-                if (a.norm_dtype == B200Q_F32) load8((const float*)w + e0, wv);
-                else load8((const __nv_bfloat16*)w + e0, wv);
+                    for (int m = kLanes / 2; m; m >>= 1) ss += __shfl_xor_sync(~0u, ss, m);
+                    const float r = rsqrtf(ss * (1.f / D) + a.eps);
+                    float wv[8];
+                    if (a.norm_dtype == B200Q_F32) { widen(raw4((const float*)w + ea), wv); widen(raw4((const float*)w + eb), wv + 4); }
+                    else { widen(raw4((const __nv_bfloat16*)w + ea), wv); widen(raw4((const __nv_bfloat16*)w + eb), wv + 4); }
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[u][j] = x[u][j] * r * wv[j];
-            }
-            if (a.rope) {
-                if (INTERLEAVED) {
-                    if (live && !is_v && e0 < a.rope) {
+                    for (int j = 0; j < 8; j++) y[j] = y[j] * r * wv[j];
+                }
+                if (turned) {
+                    const float c[4] = {c0.x, c0.z, c1.x, c1.z}, s[4] = {c0.y, c0.w, c1.y, c1.w};
 #pragma unroll
-                        for (int j = 0; j < 8; j += 2) {
-                            const float2 v = cs[(e0 + j) >> 1];
-                            const float p = x[u][j], c = x[u][j + 1];
-                            x[u][j] = p * v.x - c * v.y;
-                            x[u][j + 1] = c * v.x + p * v.y;
-                        }
-                    }
-                } else {
-                    // rope % 16 == 0: a lane's eight values lie in one half, their partners in one other lane
-                    const bool turned = e0 < a.rope, low = e0 < half;
-                    const int from = turned ? lane + (low ? half : -half) / 8 : lane;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float o = __shfl_sync(~0u, x[u][j], from);
-                        if (live && !is_v && turned) {
-                            const float2 v = cs[low ? e0 + j : e0 - half + j];
-                            x[u][j] = x[u][j] * v.x + (low ? -o : o) * v.y;
-                        }
+                    for (int j = 0; j < 4; j++) {
+                        const int i0 = INTERLEAVED ? 2 * j : j, i1 = INTERLEAVED ? 2 * j + 1 : j + 4;
+                        const float p = y[i0], q = y[i1];
+                        y[i0] = p * c[j] - q * s[j];
+                        y[i1] = q * c[j] + p * s[j];
                     }
                 }
             }
-            if (!live) continue;
-            __nv_bfloat162 o[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) o[j] = __floats2bfloat162_rn(x[u][2 * j], x[u][2 * j + 1]);   // the cache's type
-            if (is_q) *(uint4*)(a.qo + t * a.ldo + h * D + e0) = *(uint4*)o;
-            else if (stored) {
-                const int hk = is_v ? h - a.hq - a.hkv : h - a.hq;
-                __nv_bfloat16* c = (is_v ? a.vp + page * a.v_stride : a.kp + page * a.k_stride);
-                *(uint4*)(c + (((int64_t)hk << a.page_log2) + (pos & ((1 << a.page_log2) - 1))) * D + e0) = *(uint4*)o;
-            }
+            if (!live || (!is_q && !stored)) continue;
+            __nv_bfloat16* o = is_q ? a.qo + t * a.ldo + h * D
+                                    : (is_v ? a.vp + page * a.v_stride : a.kp + page * a.k_stride) + (((int64_t)h * D) << a.page_log2) + slot;
+            store4(o + ea, y);
+            store4(o + eb, y + 4);
         }
     }
     pdl_trigger();
@@ -173,14 +189,15 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv_append_k(AppendArgs a) {
 
 template <typename T, int D>
 static cudaError_t launch_append(const AppendArgs& a, int interleaved, cudaStream_t s) {
-    constexpr int kHeads = 32 / (D / 8), U = 3;
-    // few tokens: a token's heads over several CTAs, until each warp has one load or there are two CTAs an SM
-    const int loads = (a.hq + 2 * a.hkv + kHeads - 1) / kHeads, most = (loads + kAppendWarps - 1) / kAppendWarps;
-    int split = 1;
-    while (split < most && (int64_t)a.rows * split < 2 * 148) split++;
-    const dim3 grid((unsigned)a.rows, (unsigned)split);
-    return interleaved ? launch(kv_append_k<T, D, true, U>, grid, dim3(kAppendWarps * 32), 0, s, a)
-                       : launch(kv_append_k<T, D, false, U>, grid, dim3(kAppendWarps * 32), 0, s, a);
+    constexpr int kHeads = 32 / (D / 8);
+    // a row over so many warps that each has kLoads loads; with few rows more, until each has one
+    const int loads = (a.hq + kHeads - 1) / kHeads + 2 * ((a.hkv + kHeads - 1) / kHeads);
+    int64_t parts = (loads + Raw<T>::kLoads - 1) / Raw<T>::kLoads;
+    const int64_t fill = (int64_t)device_sms() * 2 * kAppendWarps / a.rows;
+    if (parts < fill) parts = fill < loads ? fill : loads;
+    const dim3 grid((unsigned)(((int64_t)a.rows * parts + kAppendWarps - 1) / kAppendWarps));
+    return interleaved ? launch(kv_append_k<T, D, true>, grid, dim3(kAppendWarps * 32), 0, s, a, (int)parts)
+                       : launch(kv_append_k<T, D, false>, grid, dim3(kAppendWarps * 32), 0, s, a, (int)parts);
 }
 
 }  // namespace b200q

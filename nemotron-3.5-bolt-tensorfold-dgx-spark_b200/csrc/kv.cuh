@@ -16,6 +16,8 @@ struct KvSeqs {
     int width, batch;
 };
 
+int device_sms();   // SMs of the current device (core.cu)
+
 inline bool kv_page_ok(int page) { return page >= 16 && page <= 256 && (page & (page - 1)) == 0; }
 inline int log2_of(int v) { int l = 0; while ((1 << l) < v) l++; return l; }
 inline bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
