@@ -61,7 +61,7 @@ constexpr int kUnit = 16;                    // keys a unit
 constexpr int kRing = 128 * 1024;            // bytes of units in flight
 constexpr int kMaxCtas = 160;                // shares the workspace holds
 constexpr int kJoin = 8;                     // accumulator fragments a join pass moves per warp (32 KB in all)
-constexpr int kMinUnits = 8;                 // a share is not smaller: one unit a warp
+constexpr int kMinUnits = 16;                // a share is not smaller: two units a warp (one: 11.7 us for a short call, not 10.3)
 
 template <int D, int NT>
 struct Shape {
@@ -244,7 +244,9 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
     bool dead = false;
 
     if (warp == kWarps) {
-        // ---------------------------------------------------------------- producer
+        // ---------------------------------------------------------------- producer: eight units at a time, a lane each
+        // (one lane for all took 170 ns a unit, the time of 8 KB at the full rate).  A unit's stage was last that of the
+        // unit NS >= 16 before it, so no lane waits for what another lane of its eight has yet to issue.
         bool bad_page = false;
         int issued = 0;
         for (long long at = begin; at < end; at = p.to) {
@@ -256,31 +258,33 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
             for (int i0 = 0; i0 < n; i0 += 32) {
                 const int mine = next;
                 if (i0 + 32 + lane < n) next = tab[((u0 + i0 + 32 + lane) * kUnit) >> a.page_log2];   // a round ahead
-                for (int i = 0; i < min(32, n - i0); i++) {
-                    int page = __shfl_sync(~0u, mine, i);
-                    if (page < 0 || page >= a.pages) { bad_page = true; page = a.pages; }   // past the end: TMA fills zeros
-                    const int o = ordinal + i0 + i, st = o % NS;
-                    if (lane == 0 && !dead) {
-                        if (!tc_mbar_wait(empty + st * 8, (o / NS & 1) ^ 1)) dead = true;
-                        else {
-                            const uint32_t dst = ring + st * S::kBytes, bar = full + st * 8;
-                            const int row = ((u0 + i0 + i) * kUnit) & ((1 << a.page_log2) - 1);
-                            tc_mbar_arrive_tx(bar, S::kBytes);
-                            tma_kv(dst, &mk, row, p.h, page, bar);
-                            tma_kv(dst + S::kBytes / 2, &mv, row, p.h, page, bar);
-                            issued = o + 1;
-                        }
+#pragma unroll
+                for (int k = 0; k < 32; k += kWarps) {
+                    const int i = i0 + k + lane;
+                    int page = __shfl_sync(~0u, mine, k + (lane & 7));
+                    const int o = ordinal + i, st = o % NS;
+                    const bool live = lane < kWarps && i < n && !dead;
+                    if (live && !tc_mbar_wait(empty + st * 8, (o / NS & 1) ^ 1)) dead = true;
+                    __syncwarp();
+                    if (live && !dead) {
+                        if (page < 0 || page >= a.pages) { bad_page = true; page = a.pages; }   // past the end: TMA fills zeros
+                        const uint32_t dst = ring + st * S::kBytes, bar = full + st * 8;
+                        const int row = ((u0 + i) * kUnit) & ((1 << a.page_log2) - 1);
+                        tc_mbar_arrive_tx(bar, S::kBytes);
+                        tma_kv(dst, &mk, row, p.h, page, bar);
+                        tma_kv(dst + S::kBytes / 2, &mv, row, p.h, page, bar);
+                        issued = o + 1;
                     }
+                    dead = __any_sync(~0u, dead);
                 }
             }
             ordinal += n;
         }
-        if (lane == 0) {
-            if (dead) atomicOr(&g_attn_error, 1);
-            // the last copies have landed before the block ends, whatever became of their readers
-            for (int o = max(0, issued - NS); o < issued; o++) tc_mbar_wait(full + (o % NS) * 8, o / NS & 1);
-            if (bad_page) atomicOr(&g_attn_error, 2);
-        }
+        if (dead && lane == 0) atomicOr(&g_attn_error, 1);
+        if (__any_sync(~0u, bad_page) && lane == 0) atomicOr(&g_attn_error, 2);
+        // the last copies have landed before the block ends, whatever became of their readers
+        issued = __reduce_max_sync(~0u, issued);
+        for (int o = max(0, issued - NS) + lane; o < issued; o += 32) tc_mbar_wait(full + (o % NS) * 8, o / NS & 1);
         return;
     }
 
