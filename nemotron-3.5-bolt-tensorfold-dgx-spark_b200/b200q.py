@@ -7,7 +7,6 @@ and calling the sm_100a kernels through ctypes.  Errors raise B200QError with li
 returns void and logs; its C ABI returns -1/-3).  There is no CPU fallback: without libb200q.so, or without a GPU,
 every operator raises.
 """
-import contextlib
 import ctypes
 import functools
 import json
@@ -625,12 +624,17 @@ def _heads(t, name, dev, dtype, d):
     return n, h, s[0] if n > 1 else h * d
 
 
-_HERE = contextlib.nullcontext()
+# the current stream of a device as an address: torch.cuda.current_stream(dev).cuda_stream without the Stream object,
+# whose making takes longer (3 us) than the rest of a call's checks
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
-def _on(dev):
-    """a context in which device `dev` is the current one"""
-    return _HERE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+def _call(dev, fn, *args):
+    """fn(*args, the current stream of device dev), with dev as the current device"""
+    if dev == torch.cuda.current_device():
+        return fn(*args, _raw_stream(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, _raw_stream(dev))
 
 
 def k_kv_append(q, k, v, k_pages, v_pages, table, lens, cu, inv_freq=None, interleaved=False, q_norm=None, k_norm=None,
@@ -673,18 +677,16 @@ def k_kv_append(q, k, v, k_pages, v_pages, table, lens, cu, inv_freq=None, inter
         raise B200QError(EINVAL, "q_norm and k_norm must have one dtype")
     if rows == 0:
         return q_out
-    with _on(dev):
-        st = lib().b200q_kv_append(kv, qp, k.data_ptr(), v.data_ptr(), F32 if dt is torch.float32 else BF16, ldq, ldk, ldv, rows,
-                                   hq, fp, rope, 1 if interleaved else 0, norms[0], norms[1], norm_dtype, eps, op, ldo,
-                                   torch.cuda.current_stream().cuda_stream)
+    st = _call(dev, lib().b200q_kv_append, kv, qp, k.data_ptr(), v.data_ptr(), F32 if dt is torch.float32 else BF16, ldq, ldk,
+               ldv, rows, hq, fp, rope, 1 if interleaved else 0, norms[0], norms[1], norm_dtype, eps, op, ldo)
     _check(st, "k_kv_append")
     return q_out
 
 
 @functools.lru_cache(maxsize=1024)
 def _attn_workspace(name, dev, *sizes):
-    with _on(dev):   # the prompt form's depends on the device's SMs
-        return getattr(lib(), name)(*sizes)
+    with torch.cuda.device(dev):   # the prompt form's depends on the device's SMs
+        return max(getattr(lib(), f"b200q_{name}_workspace_bytes")(*sizes), 16)
 
 
 def _attend(name, q, k_pages, v_pages, table, lens, cu, max_rows, scale, softcap, window, out):
@@ -699,16 +701,15 @@ def _attend(name, q, k_pages, v_pages, table, lens, cu, max_rows, scale, softcap
             raise B200QError(EINVAL, "out must have q's shape")
     if rows == 0:
         return out
-    with _on(dev):
-        if name == "attn_decode":
-            fn, nb = lib().b200q_attn_decode, _attn_workspace("b200q_attn_decode_workspace_bytes", dev, hq, hkv, d, max_rows)
-        else:
-            fn, nb = lib().b200q_attn_prompt, _attn_workspace("b200q_attn_prompt_workspace_bytes", dev, hq, hkv, d, rows,
-                                                              max_rows, batch)
-        # scratch of this call alone: calls on other streams, and captured ones, have their own
-        ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=k_pages.device)
-        st = fn(kv, q.data_ptr(), ldq, rows, hq, max_rows, d ** -0.5 if scale is None else scale, softcap, window,
-                out.data_ptr(), ldo, ws.data_ptr(), nb, torch.cuda.current_stream().cuda_stream)
+    L = lib()
+    if name == "attn_decode":
+        fn, nb = L.b200q_attn_decode, _attn_workspace(name, dev, hq, hkv, d, max_rows)
+    else:
+        fn, nb = L.b200q_attn_prompt, _attn_workspace(name, dev, hq, hkv, d, rows, max_rows, batch)
+    # scratch of this call alone: calls on other streams, and captured ones, have their own
+    ws = torch.empty(nb, dtype=torch.uint8, device=k_pages.device)
+    st = _call(dev, fn, kv, q.data_ptr(), ldq, rows, hq, max_rows, d ** -0.5 if scale is None else scale, softcap, window,
+               out.data_ptr(), ldo, ws.data_ptr(), nb)
     _check(st, name)
     return out
 

@@ -1,5 +1,6 @@
 // Shared pieces of the paged attention kernels: their arguments, the score's scaling, the cache's tensor maps.
 #pragma once
+#include <atomic>
 #include <climits>
 #include <cmath>
 
@@ -47,6 +48,19 @@ __device__ __forceinline__ void tma_kv(uint32_t dst, const CUtensorMap* m, int r
 
 // the tensor map of one side of the cache: dims (64, page, d / 64, heads, pages), box (64, box_rows, box_blocks, 1, 1)
 bool kv_tensor_map(CUtensorMap* m, const void* pages, int64_t stride, const b200q_paged& kv, int box_rows, int box_blocks);
+
+// a kernel's dynamic shared memory allowed once a device
+struct SmemOptIn {
+    std::atomic<uint64_t> done{0};
+    cudaError_t allow(const void* kernel, size_t bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess || (dev < 64 && (done.load() >> dev & 1))) return e;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e == cudaSuccess && dev < 64) done |= (uint64_t)1 << dev;
+        return e;
+    }
+};
 
 // the checks both forms share
 inline bool attn_ok(const b200q_paged* kv, const void* q, int64_t ldq, int rows, int hq, int max_rows, float scale, float softcap,

@@ -58,23 +58,24 @@ namespace {
 
 constexpr int kWarps = 8;                    // consumer warps
 constexpr int kUnit = 16;                    // keys a unit
-constexpr int kRing = 128 * 1024;            // bytes of units in flight
 constexpr int kMaxCtas = 160;                // shares the workspace holds
-constexpr int kJoin = 8;                     // accumulator fragments a join pass moves per warp (32 KB in all)
 constexpr int kMinUnits = 16;                // a share is not smaller: two units a warp (one: 11.7 us for a short call, not 10.3)
 
 template <int D, int NT>
 struct Shape {
     static constexpr int kRows = 8 * NT;                     // rows of a row block
     static constexpr int kBytes = kUnit * D * 4;             // a unit: K [D / 64][16][128 B], then V
-    static constexpr int kStages = kRing / kBytes;           // a multiple of kWarps: a warp meets its own stages only
+    // 128 KB: 5 % slower at 64 sequences of 6000 keys
+    static constexpr int kStages = 192 * 1024 / kBytes;
+    // A warp meets its own stages only.  Otherwise one could wait for a stage's next fill before its last has landed, and a
+    // wait for the parity after next returns at once.
+    static_assert(kStages % kWarps == 0 && kStages >= 2 * kWarps, "ring");
+    static constexpr int kRing = kStages * kBytes;
     static constexpr int kFrags = D / 16 * NT;               // accumulator fragments (16 x 8) of a warp
-    static constexpr size_t kQ = (size_t)kRows * D * 2;
+    static constexpr int kJoin = NT == 1 ? kFrags : 4;       // those that a pass of the join moves
+    static constexpr int kQ = kRows * D * 2, kJ = kWarps * kJoin * 512, kMix = kQ > kJ ? kQ : kJ;   // Q, then the join: one place
     static constexpr size_t kSlot = (size_t)kRows * (D + 2); // floats of a partial: O [rows][D], m [rows], sum [rows]
-    static size_t smem(int batch) {
-        return 1024 + kRing + kQ + (size_t)kWarps * kJoin * 512 + (size_t)kWarps * kRows * 8 + kStages * 16 +
-               (size_t)kRows * 8 + (size_t)(batch + 1) * 8;
-    }
+    static constexpr size_t kSmem = 1024 + kRing + kMix + (size_t)kWarps * kRows * 8 + kStages * 16;
 };
 
 struct Desc {   // what a share left to join: n partials of rows row0 .. of a sequence starting at row cu0, kv head h
@@ -128,65 +129,70 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// the line of units: pre[b] counts those of the sequences before b
-struct Line {
-    const long long* pre;
-    int batch;
-};
-// One CTA's next piece: a row block (b, h, rb) and its units from .. to - 1 (counted from the block's first), cut by the
-// share's end.  at: the line's position of the piece, advanced past it.
-struct Piece {
+// Where a CTA stands on the line: a row block (b, h, rb), its keys, the line's position of its first unit
+template <int ROWS>
+struct Cursor {
     int b, h, rb, cu0, r, len;
     Span s;
-    long long begin, end;    // the row block on the line
-    long long from, to;      // the piece on the line
-};
-template <int ROWS>
-__device__ __forceinline__ void next_piece(const AttnArgs& a, const Line& l, int nrb, long long at, long long stop, Piece& p) {
-    int lo = 0, hi = l.batch - 1;   // the last b with pre[b] <= at: sequences without units are skipped
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (l.pre[mid] <= at) lo = mid; else hi = mid - 1;
+    long long begin;
+    __device__ __forceinline__ int cost() const { return max(s.n, 1); }   // a block that sees no key still writes its zeros
+    __device__ __forceinline__ bool block(const AttnArgs& a, int nrb) {
+        return rb < nrb && row_block<ROWS>(r, len, rb, a.group, a.window, s);
     }
-    p.b = lo;
-    seq_sizes(a, lo, p.cu0, p.r, p.len);
-    const long long a_head = (l.pre[lo + 1] - l.pre[lo]) / a.hkv;
-    long long rest = at - l.pre[lo];
-    p.h = (int)(rest / a_head);
-    rest -= p.h * a_head;
-    long long before = 0;
-    for (p.rb = 0; p.rb < nrb; p.rb++) {
-        if (!row_block<ROWS>(p.r, p.len, p.rb, a.group, a.window, p.s)) break;
-        const int c = max(p.s.n, 1);
-        if (rest < before + c) {
-            p.begin = l.pre[lo] + p.h * a_head + before;
-            p.end = p.begin + c;
-            break;
+    // to sequence b's block that holds the line's position `at`: b starts at `first`, each of its heads has a_head units
+    __device__ __forceinline__ void seek(const AttnArgs& a, int nrb, long long first, long long a_head, long long at) {
+        const long long rest = at - first;
+        h = a_head < (1 << 21) ? (int)((unsigned)rest / (unsigned)a_head) : (int)(rest / a_head);   // below 2^31: <= 1024 heads
+        begin = first + h * a_head;
+        for (rb = 0; block(a, nrb) && at >= begin + cost(); rb++) begin += cost();
+    }
+    __device__ __forceinline__ void advance(const AttnArgs& a, int nrb) {
+        begin += cost();
+        rb++;
+        if (block(a, nrb)) return;
+        rb = 0;
+        if (++h == a.hkv) {
+            h = 0;
+            do seq_sizes(a, ++b, cu0, r, len);
+            while (r == 0);
         }
-        before += c;
+        block(a, nrb);
     }
-    p.from = at;
-    p.to = min(stop, p.end);
-}
+};
 
-__device__ __forceinline__ long long share_start(long long total, int k, int shares) { return total * k / shares; }
+// shares of per or per + 1 units
+struct Shares {
+    long long per;
+    int more;   // the first `more` shares have one unit more
+    __device__ __forceinline__ Shares(long long total, int n) {
+        per = total < (1ll << 32) ? (long long)((unsigned)total / (unsigned)n) : total / n;
+        more = (int)(total - per * n);
+    }
+    __device__ __forceinline__ long long start(int k) const { return per * k + min(k, more); }
+    __device__ __forceinline__ int of(long long at) const {   // the share that holds position `at`
+        int k = (int)(total_below(at) ? (unsigned)at / (unsigned)(per + 1) : at / (per + 1));
+        while (start(k + 1) <= at) k++;
+        return k;
+    }
+    static __device__ __forceinline__ bool total_below(long long at) { return at < (1ll << 32); }
+};
 
 template <int D, int NT>
 __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
 attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, AttnArgs a) {
     using S = Shape<D, NT>;
-    constexpr int RB = S::kRows, NS = S::kStages;
+    constexpr int RB = S::kRows, NS = S::kStages, kRing = S::kRing, kJoin = S::kJoin;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw), ring = (raw + 1023) & ~1023u;
     uint8_t* base = smem_raw + (ring - raw);
     uint2* qs = (uint2*)(base + kRing);                                   // Q fragments [D / 16][NT][32]
-    float4* jo = (float4*)(base + kRing + S::kQ);                         // join: [kWarps][kJoin][32]
-    float* jm = (float*)(base + kRing + S::kQ + kWarps * kJoin * 512);    // join: m [kWarps][RB], then sums
+    float4* jo = (float4*)(base + kRing);                                 // join: [kWarps][kJoin][32], once Q is done with
+    float* jm = (float*)(base + kRing + S::kMix);                         // join: m [kWarps][RB], then sums
     float* jl = jm + kWarps * RB;
-    float* jt = jl + kWarps * RB;                                          // joined m [RB], sum [RB]
-    const uint32_t full = ring + kRing + (uint32_t)S::kQ + kWarps * kJoin * 512 + (kWarps + 1) * RB * 8, empty = full + NS * 8;
-    long long* pre = (long long*)(base + (empty + NS * 8 - ring));
-    __shared__ long long warp_sum[kWarps + 1];
+    const uint32_t full = ring + kRing + S::kMix + kWarps * RB * 8, empty = full + NS * 8;
+    constexpr int kAll = (kWarps + 1) * 32;
+    __shared__ long long warp_sum[kWarps + 1], start[2];   // start: the units before the share's first sequence, those of a head
+    __shared__ int start_seq[4];                            // the sequence and its sizes
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
@@ -198,37 +204,37 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
     pdl_wait();
     pdl_trigger();
 
-    // the line: an exclusive sum of the sequences' units, 288 sequences at a time
+    // the line: an exclusive sum of the sequences' units, kAll sequences at a time
     const int nrb = (a.max_rows * a.group + RB - 1) / RB;
-    long long carry = 0;
-    if (tid == 0) pre[0] = 0;
-    for (int b0 = 0; b0 < a.s.batch; b0 += (kWarps + 1) * 32) {
+    long long units, below;   // of sequence b0 + tid: those of a head, those of the sequences before
+    int cu0 = 0, r = 0, len = 0;
+    auto scan = [&](int b0, long long carry, bool report) {
         const int b = b0 + tid;
-        long long c = 0;
+        units = 0;
         if (b < a.s.batch) {
-            int cu0, r, len;
             Span s;
             seq_sizes(a, b, cu0, r, len);
-            for (int rb = 0; rb < nrb && row_block<RB>(r, len, rb, a.group, a.window, s); rb++) c += max(s.n, 1);
-            c *= a.hkv;
-            if (blockIdx.x == 0 && (r > a.max_rows || len != a.s.lens[b])) atomicOr(&g_attn_error, r > a.max_rows ? 4 : 2);
+            for (int rb = 0; rb < nrb && row_block<RB>(r, len, rb, a.group, a.window, s); rb++) units += max(s.n, 1);
+            if (report && (r > a.max_rows || len != a.s.lens[b])) atomicOr(&g_attn_error, r > a.max_rows ? 4 : 2);
         }
-        long long sum = c;
+        long long sum = units * a.hkv;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long v = __shfl_up_sync(~0u, sum, o);
             if (lane >= o) sum += v;
         }
+        __syncthreads();   // the sums of the round before have been read
         if (lane == 31) warp_sum[warp] = sum;
         __syncthreads();
-        long long below = carry;
+        below = carry + sum - units * a.hkv;
         for (int w = 0; w <= kWarps; w++) {
             if (w < warp) below += warp_sum[w];
             carry += warp_sum[w];
         }
-        if (b < a.s.batch) pre[b + 1] = below + sum;
-        __syncthreads();
-    }
+        return carry;
+    };
+    long long carry = 0;
+    for (int b0 = 0; b0 < a.s.batch; b0 += kAll) carry = scan(b0, carry, blockIdx.x == 0);
     const long long total = carry;
     const int shares = (int)min((long long)gridDim.x, (total + kMinUnits - 1) / kMinUnits);
     Desc* desc = (Desc*)a.ws;
@@ -237,9 +243,21 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
         if (tid == 0) desc[blockIdx.x].n = 0;
         return;
     }
-    const long long begin = share_start(total, blockIdx.x, shares), end = share_start(total, blockIdx.x + 1, shares);
-    const Line line = {pre, a.s.batch};
-    Piece p;
+    const Shares split(total, shares);
+    const long long begin = split.start(blockIdx.x), end = split.start(blockIdx.x + 1);
+    // the sequence in which the share begins: in the round just scanned, or another scan finds it
+    carry = 0;
+    for (int b0 = 0; b0 < a.s.batch; b0 += kAll) {
+        if (a.s.batch > kAll) carry = scan(b0, carry, false);
+        if (units > 0 && below <= begin && begin < below + units * a.hkv) {
+            start[0] = below; start[1] = units;
+            start_seq[0] = b0 + tid; start_seq[1] = cu0; start_seq[2] = r; start_seq[3] = len;
+        }
+    }
+    __syncthreads();
+    Cursor<RB> p;
+    p.b = start_seq[0]; p.cu0 = start_seq[1]; p.r = start_seq[2]; p.len = start_seq[3];
+    p.seek(a, nrb, start[0], start[1], begin);
     int ordinal = 0;   // units of the share before the piece
     bool dead = false;
 
@@ -249,9 +267,8 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
         // unit NS >= 16 before it, so no lane waits for what another lane of its eight has yet to issue.
         bool bad_page = false;
         int issued = 0;
-        for (long long at = begin; at < end; at = p.to) {
-            next_piece<RB>(a, line, nrb, at, end, p);
-            const int n = p.s.n ? (int)(p.to - p.from) : 0, u0 = p.s.u0 + (int)(p.from - p.begin);
+        for (long long at = begin; at < end;) {
+            const int skip = (int)(at - p.begin), n = p.s.n ? (int)min((long long)p.s.n, end - p.begin) - skip : 0, u0 = p.s.u0 + skip;
             const int* tab = a.s.table + p.b * a.s.ldt;
             int next = 0;
             if (lane < n) next = tab[((u0 + lane) * kUnit) >> a.page_log2];
@@ -279,6 +296,8 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
                 }
             }
             ordinal += n;
+            at = p.begin + p.cost();
+            if (at < end) p.advance(a, nrb);
         }
         if (dead && lane == 0) atomicOr(&g_attn_error, 1);
         if (__any_sync(~0u, bad_page) && lane == 0) atomicOr(&g_attn_error, 2);
@@ -294,9 +313,10 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
     const uint32_t vrow = (lane & 7) + ((lane >> 4) & 1) * 8, vchunk = (lane >> 3) & 1;
     const float c = a.c;
     if (tid == 0) desc[blockIdx.x].n = 0;
-    for (long long at = begin; at < end; at = p.to) {
-        next_piece<RB>(a, line, nrb, at, end, p);
-        const int n = p.s.n ? (int)(p.to - p.from) : 0, u0 = p.s.u0 + (int)(p.from - p.begin);
+    for (long long at = begin; at < end;) {
+        // units skip .. of the row block are this share's
+        const int skip = (int)(at - p.begin), n = p.s.n ? (int)min((long long)p.s.n, end - p.begin) - skip : 0, u0 = p.s.u0 + skip;
+        const bool whole_block = skip == 0 && p.begin + p.cost() <= end;
         const int row0 = p.rb * RB, rows = min(RB, p.r * a.group - row0);
         // Q in fragment order: fragment (kk, nt), lane (g, t): values 16 kk + 2 t, + 1 and + 8, + 9 of row 8 nt + g
         consumers_sync();
@@ -422,40 +442,40 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
         }
         ordinal += n;
 
-        // join the warps: m and the sum first, then the accumulators, kJoin fragments a pass
+        // join the warps: the maxima, then the sums and accumulators scaled to the common one, kJoin fragments a pass
+        if (g == 0)
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                float x = sum[nt][j];
-                x += __shfl_xor_sync(~0u, x, 4);
-                x += __shfl_xor_sync(~0u, x, 8);
-                x += __shfl_xor_sync(~0u, x, 16);
-                if (g == 0) {
-                    jm[warp * RB + nt * 8 + t * 2 + j] = m[nt][j];
-                    jl[warp * RB + nt * 8 + t * 2 + j] = x;
-                }
-            }
+                for (int j = 0; j < 2; j++) jm[warp * RB + nt * 8 + t * 2 + j] = m[nt][j];
         consumers_sync();
-        float scale[NT][2];   // this warp's part of the joined scale, for this lane's columns
+        float scale[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int row = nt * 8 + t * 2 + j;
-                float x = -INFINITY, y = 0.f;
+                float x = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < kWarps; w++) x = fmaxf(x, jm[w * RB + row]);
-                const float z = x == -INFINITY ? 0.f : x;
-#pragma unroll
-                for (int w = 0; w < kWarps; w++) y += jl[w * RB + row] * ex2(jm[w * RB + row] - z);
-                scale[nt][j] = ex2(m[nt][j] - z);
-                if (tid < 4) { jt[row] = x; jt[RB + row] = y; }
+                scale[nt][j] = ex2(m[nt][j] - (x == -INFINITY ? 0.f : x));
+                float y = sum[nt][j] * scale[nt][j];
+                y += __shfl_xor_sync(~0u, y, 4);
+                y += __shfl_xor_sync(~0u, y, 8);
+                y += __shfl_xor_sync(~0u, y, 16);
+                if (g == 0) jl[warp * RB + row] = y;
+                m[nt][j] = x;
             }
-        const bool complete = p.from == p.begin && p.to == p.end;
-        float* slot = slots + ((size_t)blockIdx.x * 2 + (p.from == p.begin ? 1 : 0)) * S::kSlot;
+        auto row_sum = [&](int row) {
+            float y = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) y += jl[w * RB + row];
+            return y;
+        };
+        float* slot = slots + ((size_t)blockIdx.x * 2 + (skip == 0 ? 1 : 0)) * S::kSlot;
 #pragma unroll
         for (int pass = 0; pass < (S::kFrags + kJoin - 1) / kJoin; pass++) {
+            if (pass) consumers_sync();
 #pragma unroll
             for (int k = 0; k < kJoin; k++) {
                 const int f = pass * kJoin + k;
@@ -466,7 +486,7 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
             }
             consumers_sync();
             const int f = pass * kJoin + warp;
-            if (f < S::kFrags) {
+            if (warp < kJoin && f < S::kFrags) {
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int w = 0; w < kWarps; w++) {
@@ -474,8 +494,8 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
                     v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
                 }
                 const int d0 = f / NT * 16, r0 = f % NT * 8;
-                if (complete) {
-                    const float l0 = jt[RB + r0 + t * 2], l1 = jt[RB + r0 + t * 2 + 1];
+                if (whole_block) {
+                    const float l0 = row_sum(r0 + t * 2), l1 = row_sum(r0 + t * 2 + 1);
                     const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;   // no key seen: zeros
                     const uint32_t lo = transpose8(pack_bf16(v.x * i0, v.y * i1)), hi = transpose8(pack_bf16(v.z * i0, v.w * i1));
                     if (r0 + g < rows) {
@@ -490,72 +510,108 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
                     s0[0] = v.x; s0[D] = v.y; s0[8] = v.z; s0[D + 8] = v.w;
                 }
             }
-            consumers_sync();
         }
-        if (!complete) {
-            if (tid < 2 * RB) slot[RB * D + tid] = jt[tid];
-            if (tid == 0 && p.from == p.begin) {
-                const long long last = p.end - 1;
-                int k = (int)(last * shares / total);
-                while (share_start(total, k + 1, shares) <= last) k++;
+        if (!whole_block) {
+            if (warp == 0 && g == 0)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) slot[RB * D + nt * 8 + t * 2 + j] = m[nt][j];
+            if (tid >= 32 && tid < 32 + RB) slot[RB * D + RB + tid - 32] = row_sum(tid - 32);
+            if (tid == 0 && skip == 0) {
                 Desc& d = desc[blockIdx.x];
-                d.n = k - blockIdx.x + 1;
+                d.n = split.of(p.begin + p.cost() - 1) - blockIdx.x + 1;
                 d.cu0 = p.cu0; d.row0 = row0; d.nrows = rows; d.h = p.h;
             }
         }
+        at = p.begin + p.cost();
+        if (at < end) p.advance(a, nrb);
     }
 }
 
-// the row blocks that a share's end cut: partial 0 is the share's last, the others the first of the shares after it
+// The row blocks that a share's end cut: partial 0 is the share's last, the others the first of the shares after it.  A
+// row's partials are dealt to as many of the eight warps as rows leave it, their sums added in warp order.
 template <int D, int NT>
-__global__ void __launch_bounds__(256) attn_join_k(AttnArgs a) {
+__global__ void __launch_bounds__(256, 4) attn_join_k(AttnArgs a) {
     using S = Shape<D, NT>;
-    constexpr int RB = S::kRows, V = D / 32;
-    __shared__ float weight[8][kMaxCtas];
+    constexpr int RB = S::kRows, V = D / 32, kAhead = 8;
+    __shared__ float weight[8][kMaxCtas], part[8][D];
     pdl_wait();
     pdl_trigger();
-    const Desc d = ((const Desc*)a.ws)[blockIdx.x];
-    if (d.n <= 0) return;
     const float* slots = (const float*)((const uint8_t*)a.ws + kMaxCtas * sizeof(Desc));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     auto slot = [&](int i) { return slots + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * S::kSlot; };
-    for (int r = warp; r < d.nrows; r += 8) {
-        float top = -INFINITY, sum = 0.f;
-        for (int i = lane; i < d.n; i += 32) top = fmaxf(top, slot(i)[RB * D + r]);
+    const int most = min(RB, a.max_rows * a.group), each = most >= 5 ? 1 : most >= 3 ? 2 : most == 2 ? 4 : 8;   // warps a row
+    const int mine = warp % each;
+    const Desc d = ((const Desc*)a.ws)[blockIdx.x];
+    if (d.n <= 0) return;
+    float x[kAhead][V], m0 = 0.f, l0 = 0.f;
+    auto load = [&](int r, int i0) {
 #pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        const float z = top == -INFINITY ? 0.f : top;
-        for (int i = lane; i < d.n; i += 32) {
-            const float w = ex2(slot(i)[RB * D + r] - z);
-            weight[warp][i] = w;
-            sum += w * slot(i)[RB * D + RB + r];
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-        __syncwarp();
-        float acc[V] = {};
-#pragma unroll 4
-        for (int i = 0; i < d.n; i++) {
+        for (int k = 0; k < kAhead; k++) {
+            const int i = i0 + k * each;
+            if (i >= d.n) continue;
             const float* p = slot(i) + r * D + lane * V;
-            const float w = weight[warp][i];
-            float x[V];
-            if (V == 4) *(float4*)x = *(const float4*)p; else *(float2*)x = *(const float2*)p;
-#pragma unroll
-            for (int j = 0; j < V; j++) acc[j] = fmaf(w, x[j], acc[j]);
+            if (V == 4) *(float4*)x[k] = *(const float4*)p; else *(float2*)x[k] = *(const float2*)p;
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int rr = d.row0 + r, tok = rr / a.group;
-        uint32_t* dst = (uint32_t*)(a.out + (d.cu0 + tok) * a.ldo + (int64_t)(d.h * a.group + rr - tok * a.group) * D + lane * V);
+    };
+    for (int r0 = 0; r0 < d.nrows; r0 += 8 / each) {
+        const int r = r0 + warp / each;
+        const bool live = r < d.nrows;
+        float acc[V] = {}, sum = 0.f;
+        if (live) {
+            load(r, mine);   // beside the weights
+            if (lane < d.n) { m0 = slot(lane)[RB * D + r]; l0 = slot(lane)[RB * D + RB + r]; }
+            float top = lane < d.n ? m0 : -INFINITY;
+            for (int i = lane + 32; i < d.n; i += 32) top = fmaxf(top, slot(i)[RB * D + r]);
 #pragma unroll
-        for (int j = 0; j < V / 2; j++) dst[j] = pack_bf16(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+            const float z = top == -INFINITY ? 0.f : top;
+            for (int i = lane; i < d.n; i += 32) {
+                const float w = ex2((i < 32 ? m0 : slot(i)[RB * D + r]) - z);
+                weight[warp][i] = w;
+                sum += w * (i < 32 ? l0 : slot(i)[RB * D + RB + r]);
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+            __syncwarp();
+            for (int i0 = mine; i0 < d.n; i0 += kAhead * each) {
+                if (i0 != mine) load(r, i0);
+#pragma unroll
+                for (int k = 0; k < kAhead; k++) {
+                    const int i = i0 + k * each;
+                    if (i >= d.n) break;
+#pragma unroll
+                    for (int j = 0; j < V; j++) acc[j] = fmaf(weight[warp][i], x[k][j], acc[j]);
+                }
+            }
+        }
+        if (each > 1) {
+#pragma unroll
+            for (int j = 0; j < V; j++) part[warp][lane * V + j] = acc[j];
+            __syncthreads();
+            if (live && mine == 0)
+                for (int w = 1; w < each; w++)
+#pragma unroll
+                    for (int j = 0; j < V; j++) acc[j] += part[warp + w][lane * V + j];
+            __syncthreads();
+        }
+        if (live && mine == 0) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const int rr = d.row0 + r, tok = rr / a.group;
+            uint32_t* dst = (uint32_t*)(a.out + (d.cu0 + tok) * a.ldo + (int64_t)(d.h * a.group + rr - tok * a.group) * D + lane * V);
+#pragma unroll
+            for (int j = 0; j < V / 2; j++) dst[j] = pack_bf16(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+        }
         __syncwarp();
     }
 }
 
 template <int D, int NT>
 cudaError_t launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& a, cudaStream_t s) {
-    const size_t smem = Shape<D, NT>::smem(a.s.batch);
-    cudaError_t e = cudaFuncSetAttribute(attn_rows_k<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const size_t smem = Shape<D, NT>::kSmem;
+    static SmemOptIn opted;
+    cudaError_t e = opted.allow((const void*)attn_rows_k<D, NT>, smem);
     if (e != cudaSuccess) return e;
     const int ctas = min(device_sms(), kMaxCtas);
     e = launch(attn_rows_k<D, NT>, dim3(ctas), dim3((kWarps + 1) * 32), smem, s, mk, mv, a);

@@ -619,7 +619,8 @@ int key_shares(int64_t ctas) {
 template <int D>
 cudaError_t launch_prompt(const CUtensorMap& mk, const CUtensorMap& mv, const PromptArgs& p, cudaStream_t s) {
     const size_t smem = Lay<D>::smem(p.a.s.batch);
-    cudaError_t e = cudaFuncSetAttribute(attn_prompt_k<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static SmemOptIn opted;
+    cudaError_t e = opted.allow((const void*)attn_prompt_k<D>, Lay<D>::smem(4096));
     if (e != cudaSuccess) return e;
     e = launch(attn_prompt_k<D>, dim3((unsigned)(p.blocks * p.a.hkv * p.shares)), dim3(kThreads), smem, s, mk, mv, p);
     if (e != cudaSuccess || p.shares == 1) return e;

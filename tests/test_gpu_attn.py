@@ -228,3 +228,12 @@ def test_many_sequences():
     sizes[5] = (0, 10)
     run(Step(sizes, 4, 2, 64, 16), b200q.attn_decode)
     run(Step(sizes, 4, 2, 64, 16), b200q.attn_prompt)
+
+
+@pytest.mark.parametrize("d,page", [(128, 64), (64, 16)])
+@pytest.mark.parametrize("hq,hkv,rows", [(8, 8, 1), (16, 8, 8), (32, 8, 16)])
+def test_shares_longer_than_the_ring(d, page, hq, hkv, rows):
+    """every CTA walks several sequences, with far more keys than its shared memory holds at once"""
+    g = torch.Generator().manual_seed(1)
+    sizes = [(rows, int(torch.randint(2000, 6000, (), generator=g))) for _ in range(9)] + [(rows, 16), (rows, 9000)]
+    run(Step(sizes, hq, hkv, d, page, junk=math.nan), b200q.attn_decode)
