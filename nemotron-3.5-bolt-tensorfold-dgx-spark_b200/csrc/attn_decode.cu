@@ -4,11 +4,8 @@
 //
 // Bound by HBM: every key and value a row sees is read once for all rows and query heads of its kv head.
 //
-// Work.  A row block is up to 8 NT rows (row = token * group + query head of the group) of one (sequence, kv head); its
-// keys are cut into units of 16 (within one page, since pages hold 16 or more).  The units of all row blocks stand in one
-// line, and each CTA takes an equal share of the line: ragged lengths and few long sequences load every SM alike, whatever
-// the lengths on the device are.  A row block cut by a share's end leaves partial sums (fp32), which a second small kernel
-// joins in the line's order, so results do not depend on timing.
+// Work is shared as attn_line.cuh says, in units of 16 keys (within one page, since pages hold 16 or more) and row blocks
+// of 8 NT rows, a CTA an SM.
 //
 // A CTA is one producer warp, which walks the share and fills a ring of units by TMA (128-byte swizzle), and eight
 // consumer warps, which take the ring's units in turn.  Scores are formed transposed, S^T = K Q^T: 16 keys are the rows of
@@ -16,7 +13,7 @@
 // other way round would waste three quarters).  The probabilities' accumulator becomes the B operand of O^T += V^T P^T by one
 // 8 x 8 transpose (movmatrix) each; P is rounded to bf16 there, V's type: 2^-9 relative on weights that are summed with
 // independent signs, below the output's own rounding.  m, the sum and O stay in fp32.
-#include "attn.cuh"
+#include "attn_line.cuh"
 #include "tcgen05.cuh"
 
 namespace b200q {
@@ -58,7 +55,6 @@ namespace {
 
 constexpr int kWarps = 8;                    // consumer warps
 constexpr int kUnit = 16;                    // keys a unit
-constexpr int kMaxCtas = 160;                // shares the workspace holds
 constexpr int kMinUnits = 16;                // a share is not smaller: two units a warp (one: 11.7 us for a short call, not 10.3)
 
 template <int D, int NT>
@@ -74,37 +70,10 @@ struct Shape {
     static constexpr int kFrags = D / 16 * NT;               // accumulator fragments (16 x 8) of a warp
     static constexpr int kJoin = NT == 1 ? kFrags : 4;       // those that a pass of the join moves
     static constexpr int kQ = kRows * D * 2, kJ = kWarps * kJoin * 512, kMix = kQ > kJ ? kQ : kJ;   // Q, then the join: one place
-    static constexpr size_t kSlot = (size_t)kRows * (D + 2); // floats of a partial: O [rows][D], m [rows], sum [rows]
     static constexpr size_t kSmem = 1024 + kRing + kMix + (size_t)kWarps * kRows * 8 + kStages * 16;
 };
 
-struct Desc {   // what a share left to join: n partials of rows row0 .. of a sequence starting at row cu0, kv head h
-    int n, cu0, row0, nrows, h, pad[3];
-};
-
-// a row block's keys: units u0 .. u0 + n - 1 hold every key that one of its rows sees
-struct Span {
-    int u0, n, lo, hi, p0, p1;   // keys lo .. hi - 1; positions of its first and last row
-};
-template <int ROWS>
-__device__ __forceinline__ bool row_block(int r, int len, int rb, int group, int window, Span& s) {
-    const int first = rb * ROWS, all = r * group;
-    if (first >= all) return false;
-    const int last = min(first + ROWS, all) - 1;
-    s.p0 = len - r + first / group;
-    s.p1 = len - r + last / group;
-    s.hi = max(s.p1 + 1, 0);
-    s.lo = min(max(0, s.p0 - window + 1), s.hi);
-    s.u0 = s.lo / kUnit;
-    s.n = s.hi > s.lo ? (s.hi + kUnit - 1) / kUnit - s.u0 : 0;
-    return true;
-}
-
-__device__ __forceinline__ void seq_sizes(const AttnArgs& a, int b, int& cu0, int& r, int& len) {
-    cu0 = min(max(a.s.cu[b], 0), a.rows);
-    r = min(max(a.s.cu[b + 1], cu0), a.rows) - cu0;
-    len = min(max(a.s.lens[b], 0), a.s.width << a.page_log2);
-}
+using namespace line;
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -123,59 +92,7 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *(uint32_t*)&v;
-}
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-
-// Where a CTA stands on the line: a row block (b, h, rb), its keys, the line's position of its first unit
-template <int ROWS>
-struct Cursor {
-    int b, h, rb, cu0, r, len;
-    Span s;
-    long long begin;
-    __device__ __forceinline__ int cost() const { return max(s.n, 1); }   // a block that sees no key still writes its zeros
-    __device__ __forceinline__ bool block(const AttnArgs& a, int nrb) {
-        return rb < nrb && row_block<ROWS>(r, len, rb, a.group, a.window, s);
-    }
-    // to sequence b's block that holds the line's position `at`: b starts at `first`, each of its heads has a_head units
-    __device__ __forceinline__ void seek(const AttnArgs& a, int nrb, long long first, long long a_head, long long at) {
-        const long long rest = at - first;
-        h = a_head < (1 << 21) ? (int)((unsigned)rest / (unsigned)a_head) : (int)(rest / a_head);   // below 2^31: <= 1024 heads
-        begin = first + h * a_head;
-        for (rb = 0; block(a, nrb) && at >= begin + cost(); rb++) begin += cost();
-    }
-    __device__ __forceinline__ void advance(const AttnArgs& a, int nrb) {
-        begin += cost();
-        rb++;
-        if (block(a, nrb)) return;
-        rb = 0;
-        if (++h == a.hkv) {
-            h = 0;
-            do seq_sizes(a, ++b, cu0, r, len);
-            while (r == 0);
-        }
-        block(a, nrb);
-    }
-};
-
-// shares of per or per + 1 units
-struct Shares {
-    long long per;
-    int more;   // the first `more` shares have one unit more
-    __device__ __forceinline__ Shares(long long total, int n) {
-        per = total < (1ll << 32) ? (long long)((unsigned)total / (unsigned)n) : total / n;
-        more = (int)(total - per * n);
-    }
-    __device__ __forceinline__ long long start(int k) const { return per * k + min(k, more); }
-    __device__ __forceinline__ int of(long long at) const {   // the share that holds position `at`
-        int k = (int)(total_below(at) ? (unsigned)at / (unsigned)(per + 1) : at / (per + 1));
-        while (start(k + 1) <= at) k++;
-        return k;
-    }
-    static __device__ __forceinline__ bool total_below(long long at) { return at < (1ll << 32); }
-};
 
 template <int D, int NT>
 __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
@@ -191,8 +108,6 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
     float* jl = jm + kWarps * RB;
     const uint32_t full = ring + kRing + S::kMix + kWarps * RB * 8, empty = full + NS * 8;
     constexpr int kAll = (kWarps + 1) * 32;
-    __shared__ long long warp_sum[kWarps + 1], start[2];   // start: the units before the share's first sequence, those of a head
-    __shared__ int start_seq[4];                            // the sequence and its sizes
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
@@ -204,60 +119,20 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
     pdl_wait();
     pdl_trigger();
 
-    // the line: an exclusive sum of the sequences' units, kAll sequences at a time
     const int nrb = (a.max_rows * a.group + RB - 1) / RB;
-    long long units, below;   // of sequence b0 + tid: those of a head, those of the sequences before
-    int cu0 = 0, r = 0, len = 0;
-    auto scan = [&](int b0, long long carry, bool report) {
-        const int b = b0 + tid;
-        units = 0;
-        if (b < a.s.batch) {
-            Span s;
-            seq_sizes(a, b, cu0, r, len);
-            for (int rb = 0; rb < nrb && row_block<RB>(r, len, rb, a.group, a.window, s); rb++) units += max(s.n, 1);
-            if (report && (r > a.max_rows || len != a.s.lens[b])) atomicOr(&g_attn_error, r > a.max_rows ? 4 : 2);
-        }
-        long long sum = units * a.hkv;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(~0u, sum, o);
-            if (lane >= o) sum += v;
-        }
-        __syncthreads();   // the sums of the round before have been read
-        if (lane == 31) warp_sum[warp] = sum;
-        __syncthreads();
-        below = carry + sum - units * a.hkv;
-        for (int w = 0; w <= kWarps; w++) {
-            if (w < warp) below += warp_sum[w];
-            carry += warp_sum[w];
-        }
-        return carry;
-    };
-    long long carry = 0;
-    for (int b0 = 0; b0 < a.s.batch; b0 += kAll) carry = scan(b0, carry, blockIdx.x == 0);
-    const long long total = carry;
+    Scan<RB, kUnit, kAll> scan(*(typename Scan<RB, kUnit, kAll>::Shared*)base, nrb);   // in the ring, before its first fill
+    const long long total = scan.total(a, blockIdx.x == 0 ? &g_attn_error : nullptr);
     const int shares = (int)min((long long)gridDim.x, (total + kMinUnits - 1) / kMinUnits);
     Desc* desc = (Desc*)a.ws;
-    float* slots = (float*)((uint8_t*)a.ws + kMaxCtas * sizeof(Desc));
     if ((int)blockIdx.x >= shares) {
         if (tid == 0) desc[blockIdx.x].n = 0;
         return;
     }
     const Shares split(total, shares);
     const long long begin = split.start(blockIdx.x), end = split.start(blockIdx.x + 1);
-    // the sequence in which the share begins: in the round just scanned, or another scan finds it
-    carry = 0;
-    for (int b0 = 0; b0 < a.s.batch; b0 += kAll) {
-        if (a.s.batch > kAll) carry = scan(b0, carry, false);
-        if (units > 0 && below <= begin && begin < below + units * a.hkv) {
-            start[0] = below; start[1] = units;
-            start_seq[0] = b0 + tid; start_seq[1] = cu0; start_seq[2] = r; start_seq[3] = len;
-        }
-    }
+    Cursor<RB, kUnit> p = scan.seek(a, begin);
+    tc_fence_proxy_async();
     __syncthreads();
-    Cursor<RB> p;
-    p.b = start_seq[0]; p.cu0 = start_seq[1]; p.r = start_seq[2]; p.len = start_seq[3];
-    p.seek(a, nrb, start[0], start[1], begin);
     int ordinal = 0;   // units of the share before the piece
     bool dead = false;
 
@@ -296,7 +171,7 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
                 }
             }
             ordinal += n;
-            at = p.begin + p.cost();
+            at = p.end();
             if (at < end) p.advance(a, nrb);
         }
         if (dead && lane == 0) atomicOr(&g_attn_error, 1);
@@ -316,7 +191,7 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
     for (long long at = begin; at < end;) {
         // units skip .. of the row block are this share's
         const int skip = (int)(at - p.begin), n = p.s.n ? (int)min((long long)p.s.n, end - p.begin) - skip : 0, u0 = p.s.u0 + skip;
-        const bool whole_block = skip == 0 && p.begin + p.cost() <= end;
+        const bool whole_block = skip == 0 && p.end() <= end;
         const int row0 = p.rb * RB, rows = min(RB, p.r * a.group - row0);
         // Q in fragment order: fragment (kk, nt), lane (g, t): values 16 kk + 2 t, + 1 and + 8, + 9 of row 8 nt + g
         consumers_sync();
@@ -472,7 +347,7 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
             for (int w = 0; w < kWarps; w++) y += jl[w * RB + row];
             return y;
         };
-        float* slot = slots + ((size_t)blockIdx.x * 2 + (skip == 0 ? 1 : 0)) * S::kSlot;
+        float* slot = slots(a.ws) + ((size_t)blockIdx.x * 2 + (skip == 0 ? 1 : 0)) * kSlot<D, RB>;
 #pragma unroll
         for (int pass = 0; pass < (S::kFrags + kJoin - 1) / kJoin; pass++) {
             if (pass) consumers_sync();
@@ -520,90 +395,12 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
             if (tid >= 32 && tid < 32 + RB) slot[RB * D + RB + tid - 32] = row_sum(tid - 32);
             if (tid == 0 && skip == 0) {
                 Desc& d = desc[blockIdx.x];
-                d.n = split.of(p.begin + p.cost() - 1) - blockIdx.x + 1;
+                d.n = split.of(p.end() - 1) - blockIdx.x + 1;
                 d.cu0 = p.cu0; d.row0 = row0; d.nrows = rows; d.h = p.h;
             }
         }
-        at = p.begin + p.cost();
+        at = p.end();
         if (at < end) p.advance(a, nrb);
-    }
-}
-
-// The row blocks that a share's end cut: partial 0 is the share's last, the others the first of the shares after it.  A
-// row's partials are dealt to as many of the eight warps as rows leave it, their sums added in warp order.
-template <int D, int NT>
-__global__ void __launch_bounds__(256, 4) attn_join_k(AttnArgs a) {
-    using S = Shape<D, NT>;
-    constexpr int RB = S::kRows, V = D / 32, kAhead = 8;
-    __shared__ float weight[8][kMaxCtas], part[8][D];
-    pdl_wait();
-    pdl_trigger();
-    const float* slots = (const float*)((const uint8_t*)a.ws + kMaxCtas * sizeof(Desc));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    auto slot = [&](int i) { return slots + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * S::kSlot; };
-    const int most = min(RB, a.max_rows * a.group), each = most >= 5 ? 1 : most >= 3 ? 2 : most == 2 ? 4 : 8;   // warps a row
-    const int mine = warp % each;
-    const Desc d = ((const Desc*)a.ws)[blockIdx.x];
-    if (d.n <= 0) return;
-    float x[kAhead][V], m0 = 0.f, l0 = 0.f;
-    auto load = [&](int r, int i0) {
-#pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            const int i = i0 + k * each;
-            if (i >= d.n) continue;
-            const float* p = slot(i) + r * D + lane * V;
-            if (V == 4) *(float4*)x[k] = *(const float4*)p; else *(float2*)x[k] = *(const float2*)p;
-        }
-    };
-    for (int r0 = 0; r0 < d.nrows; r0 += 8 / each) {
-        const int r = r0 + warp / each;
-        const bool live = r < d.nrows;
-        float acc[V] = {}, sum = 0.f;
-        if (live) {
-            load(r, mine);   // beside the weights
-            if (lane < d.n) { m0 = slot(lane)[RB * D + r]; l0 = slot(lane)[RB * D + RB + r]; }
-            float top = lane < d.n ? m0 : -INFINITY;
-            for (int i = lane + 32; i < d.n; i += 32) top = fmaxf(top, slot(i)[RB * D + r]);
-#pragma unroll
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-            const float z = top == -INFINITY ? 0.f : top;
-            for (int i = lane; i < d.n; i += 32) {
-                const float w = ex2((i < 32 ? m0 : slot(i)[RB * D + r]) - z);
-                weight[warp][i] = w;
-                sum += w * (i < 32 ? l0 : slot(i)[RB * D + RB + r]);
-            }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-            __syncwarp();
-            for (int i0 = mine; i0 < d.n; i0 += kAhead * each) {
-                if (i0 != mine) load(r, i0);
-#pragma unroll
-                for (int k = 0; k < kAhead; k++) {
-                    const int i = i0 + k * each;
-                    if (i >= d.n) break;
-#pragma unroll
-                    for (int j = 0; j < V; j++) acc[j] = fmaf(weight[warp][i], x[k][j], acc[j]);
-                }
-            }
-        }
-        if (each > 1) {
-#pragma unroll
-            for (int j = 0; j < V; j++) part[warp][lane * V + j] = acc[j];
-            __syncthreads();
-            if (live && mine == 0)
-                for (int w = 1; w < each; w++)
-#pragma unroll
-                    for (int j = 0; j < V; j++) acc[j] += part[warp + w][lane * V + j];
-            __syncthreads();
-        }
-        if (live && mine == 0) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            const int rr = d.row0 + r, tok = rr / a.group;
-            uint32_t* dst = (uint32_t*)(a.out + (d.cu0 + tok) * a.ldo + (int64_t)(d.h * a.group + rr - tok * a.group) * D + lane * V);
-#pragma unroll
-            for (int j = 0; j < V / 2; j++) dst[j] = pack_bf16(acc[2 * j] * inv, acc[2 * j + 1] * inv);
-        }
-        __syncwarp();
     }
 }
 
@@ -613,17 +410,17 @@ cudaError_t launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const Attn
     static SmemOptIn opted;
     cudaError_t e = opted.allow((const void*)attn_rows_k<D, NT>, smem);
     if (e != cudaSuccess) return e;
-    const int ctas = min(device_sms(), kMaxCtas);
+    const int ctas = min(device_sms(), kMaxShares);
     e = launch(attn_rows_k<D, NT>, dim3(ctas), dim3((kWarps + 1) * 32), smem, s, mk, mv, a);
     if (e != cudaSuccess) return e;
-    return launch(attn_join_k<D, NT>, dim3(ctas), dim3(256), 0, s, a);
+    return launch(join_k<D, Shape<D, NT>::kRows>, dim3(ctas), dim3(256), 0, s, a);
 }
 
 int row_tiles(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
 size_t attend_ws(int hq, int hkv, int d, int max_rows) {
     const int64_t rows = (int64_t)max_rows * (hq / hkv);
-    return kMaxCtas * (sizeof(Desc) + 2 * (size_t)row_tiles(rows) * 8 * (d + 2) * sizeof(float));
+    return kMaxShares * (sizeof(Desc) + 2 * (size_t)row_tiles(rows) * 8 * (d + 2) * sizeof(float));
 }
 
 }  // namespace
