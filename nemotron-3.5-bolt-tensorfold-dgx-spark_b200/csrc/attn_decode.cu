@@ -30,7 +30,7 @@ int attn_error_read(int clear) {
     return v;
 }
 
-bool kv_tensor_map(CUtensorMap* m, const void* pages, int64_t stride, const b200q_paged& kv, int box_rows, int box_blocks) {
+bool kv_tensor_map(CUtensorMap* m, const void* pages, int64_t stride, const b200q_paged& kv, int box_rows, int box_blocks, int cols) {
     typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -43,11 +43,11 @@ bool kv_tensor_map(CUtensorMap* m, const void* pages, int64_t stride, const b200
         return (Encode)f;
     }();
     if (!encode) return false;
-    const cuuint64_t dims[5] = {64, (cuuint64_t)kv.page, (cuuint64_t)kv.d / 64, (cuuint64_t)kv.hkv, (cuuint64_t)kv.pages};
-    const cuuint64_t strides[4] = {(cuuint64_t)kv.d * 2, 128, (cuuint64_t)kv.page * kv.d * 2, (cuuint64_t)stride * 2};
-    const cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_blocks, 1, 1}, one[5] = {1, 1, 1, 1, 1};
+    const cuuint64_t dims[5] = {(cuuint64_t)cols, (cuuint64_t)kv.page, (cuuint64_t)kv.d / cols, (cuuint64_t)kv.hkv, (cuuint64_t)kv.pages};
+    const cuuint64_t strides[4] = {(cuuint64_t)kv.d * 2, (cuuint64_t)cols * 2, (cuuint64_t)kv.page * kv.d * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[5] = {(cuuint32_t)cols, (cuuint32_t)box_rows, (cuuint32_t)box_blocks, 1, 1}, one[5] = {1, 1, 1, 1, 1};
     return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(pages), dims, strides, box, one,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -442,8 +442,8 @@ int b200q_attn_decode(const b200q_paged* kv, const void* q, int64_t ldq, int row
     if (rows == 0) return B200Q_OK;
     const AttnArgs a = attn_args(*kv, q, ldq, rows, hq, max_rows, scale, softcap, window, out, ldo, workspace);
     CUtensorMap mk, mv;
-    if (!kv_tensor_map(&mk, kv->k_pages, kv->k_stride, *kv, kUnit, d / 64) ||
-        !kv_tensor_map(&mv, kv->v_pages, kv->v_stride, *kv, kUnit, d / 64))
+    if (!kv_tensor_map(&mk, kv->k_pages, kv->k_stride, *kv, kUnit, d / 64, 64) ||
+        !kv_tensor_map(&mv, kv->v_pages, kv->v_stride, *kv, kUnit, d / 64, 64))
         return status_from(cudaErrorInvalidValue);
     const cudaStream_t s = (cudaStream_t)stream;
     const int nt = row_tiles((int64_t)max_rows * a.group);
