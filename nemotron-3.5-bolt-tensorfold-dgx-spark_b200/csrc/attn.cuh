@@ -22,7 +22,6 @@ struct AttnArgs {
     float cap_in;              // softcap: scale / cap, 0: none
     int window;                // keys a row sees at most (INT_MAX / 2: no window)
     void* ws;
-    int blocks;                // row blocks of all kv heads, at most (the prompt form)
 };
 
 // The exponent of a raw score q . k: with a cap, cap * tanh(scale q.k / cap) = cap * (1 - 2 / (exp(2 y) + 1)).  The
@@ -47,9 +46,8 @@ __device__ __forceinline__ void tma_kv(uint32_t dst, const CUtensorMap* m, int r
         ::"r"(dst), "l"(m), "r"(0), "r"(row), "r"(head), "r"(page), "r"(bar) : "memory");
 }
 
-// The tensor map of one side of the cache: dims (cols, page, d / cols, heads, pages), box (cols, box_rows, box_blocks, 1,
-// 1), cols = 64 in the 128-byte swizzle or 32 in the 64-byte one.
-bool kv_tensor_map(CUtensorMap* m, const void* pages, int64_t stride, const b200q_paged& kv, int box_rows, int box_blocks, int cols);
+// the tensor map of one side of the cache: dims (64, page, d / 64, heads, pages), box (64, box_rows, box_blocks, 1, 1)
+bool kv_tensor_map(CUtensorMap* m, const void* pages, int64_t stride, const b200q_paged& kv, int box_rows, int box_blocks);
 
 // a kernel's dynamic shared memory allowed once a device
 struct SmemOptIn {

@@ -30,7 +30,7 @@ int attn_error_read(int clear) {
     return v;
 }
 
-bool kv_tensor_map(CUtensorMap* m, const void* pages, int64_t stride, const b200q_paged& kv, int box_rows, int box_blocks, int cols) {
+bool kv_tensor_map(CUtensorMap* m, const void* pages, int64_t stride, const b200q_paged& kv, int box_rows, int box_blocks) {
     typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -43,11 +43,11 @@ bool kv_tensor_map(CUtensorMap* m, const void* pages, int64_t stride, const b200
         return (Encode)f;
     }();
     if (!encode) return false;
-    const cuuint64_t dims[5] = {(cuuint64_t)cols, (cuuint64_t)kv.page, (cuuint64_t)kv.d / cols, (cuuint64_t)kv.hkv, (cuuint64_t)kv.pages};
-    const cuuint64_t strides[4] = {(cuuint64_t)kv.d * 2, (cuuint64_t)cols * 2, (cuuint64_t)kv.page * kv.d * 2, (cuuint64_t)stride * 2};
-    const cuuint32_t box[5] = {(cuuint32_t)cols, (cuuint32_t)box_rows, (cuuint32_t)box_blocks, 1, 1}, one[5] = {1, 1, 1, 1, 1};
+    const cuuint64_t dims[5] = {64, (cuuint64_t)kv.page, (cuuint64_t)kv.d / 64, (cuuint64_t)kv.hkv, (cuuint64_t)kv.pages};
+    const cuuint64_t strides[4] = {(cuuint64_t)kv.d * 2, 128, (cuuint64_t)kv.page * kv.d * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_blocks, 1, 1}, one[5] = {1, 1, 1, 1, 1};
     return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(pages), dims, strides, box, one,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -120,7 +120,7 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
     pdl_trigger();
 
     const int nrb = (a.max_rows * a.group + RB - 1) / RB;
-    Scan<RB, kUnit, kAll> scan(*(typename Scan<RB, kUnit, kAll>::Shared*)base, nrb);   // in the ring, before its first fill
+    Scan<RB, kUnit, 0, kAll> scan(*(typename Scan<RB, kUnit, 0, kAll>::Shared*)base, nrb);   // in the ring, before its first fill
     const long long total = scan.total(a, blockIdx.x == 0 ? &g_attn_error : nullptr);
     const int shares = (int)min((long long)gridDim.x, (total + kMinUnits - 1) / kMinUnits);
     Desc* desc = (Desc*)a.ws;
@@ -130,7 +130,7 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
     }
     const Shares split(total, shares);
     const long long begin = split.start(blockIdx.x), end = split.start(blockIdx.x + 1);
-    Cursor<RB, kUnit> p = scan.seek(a, begin);
+    Cursor<RB, kUnit, 0> p = scan.seek(a, begin);
     tc_fence_proxy_async();
     __syncthreads();
     int ordinal = 0;   // units of the share before the piece
@@ -143,7 +143,7 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
         bool bad_page = false;
         int issued = 0;
         for (long long at = begin; at < end;) {
-            const int skip = (int)(at - p.begin), n = p.s.n ? (int)min((long long)p.s.n, end - p.begin) - skip : 0, u0 = p.s.u0 + skip;
+            const int skip = p.from(begin), n = p.to(end) - skip, u0 = p.s.u0 + skip;
             const int* tab = a.s.table + p.b * a.s.ldt;
             int next = 0;
             if (lane < n) next = tab[((u0 + lane) * kUnit) >> a.page_log2];
@@ -190,8 +190,8 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
     if (tid == 0) desc[blockIdx.x].n = 0;
     for (long long at = begin; at < end;) {
         // units skip .. of the row block are this share's
-        const int skip = (int)(at - p.begin), n = p.s.n ? (int)min((long long)p.s.n, end - p.begin) - skip : 0, u0 = p.s.u0 + skip;
-        const bool whole_block = skip == 0 && p.end() <= end;
+        const int skip = p.from(begin), n = p.to(end) - skip, u0 = p.s.u0 + skip;
+        const bool whole_block = n == p.s.n;
         const int row0 = p.rb * RB, rows = min(RB, p.r * a.group - row0);
         // Q in fragment order: fragment (kk, nt), lane (g, t): values 16 kk + 2 t, + 1 and + 8, + 9 of row 8 nt + g
         consumers_sync();
@@ -395,7 +395,7 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
             if (tid >= 32 && tid < 32 + RB) slot[RB * D + RB + tid - 32] = row_sum(tid - 32);
             if (tid == 0 && skip == 0) {
                 Desc& d = desc[blockIdx.x];
-                d.n = split.of(p.end() - 1) - blockIdx.x + 1;
+                d.n = p.last_share(split, blockIdx.x) - blockIdx.x + 1;
                 d.cu0 = p.cu0; d.row0 = row0; d.nrows = rows; d.h = p.h;
             }
         }
@@ -442,8 +442,8 @@ int b200q_attn_decode(const b200q_paged* kv, const void* q, int64_t ldq, int row
     if (rows == 0) return B200Q_OK;
     const AttnArgs a = attn_args(*kv, q, ldq, rows, hq, max_rows, scale, softcap, window, out, ldo, workspace);
     CUtensorMap mk, mv;
-    if (!kv_tensor_map(&mk, kv->k_pages, kv->k_stride, *kv, kUnit, d / 64, 64) ||
-        !kv_tensor_map(&mv, kv->v_pages, kv->v_stride, *kv, kUnit, d / 64, 64))
+    if (!kv_tensor_map(&mk, kv->k_pages, kv->k_stride, *kv, kUnit, d / 64) ||
+        !kv_tensor_map(&mv, kv->v_pages, kv->v_stride, *kv, kUnit, d / 64))
         return status_from(cudaErrorInvalidValue);
     const cudaStream_t s = (cudaStream_t)stream;
     const int nt = row_tiles((int64_t)max_rows * a.group);

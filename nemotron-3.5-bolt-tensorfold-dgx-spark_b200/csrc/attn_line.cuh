@@ -40,7 +40,10 @@ __device__ __forceinline__ bool row_block(int r, int len, int rb, int group, int
     s.n = s.hi > s.lo ? (s.hi + UNIT - 1) / UNIT - s.u0 : 0;
     return true;
 }
-__device__ __forceinline__ int cost_of(const Span& s) { return max(s.n, 1); }   // a block that sees no key still writes zeros
+// A block's length on the line: its units (one where it sees no key: it still writes zeros) and OVER for what a block costs
+// whatever its units.
+template <int OVER>
+__device__ __forceinline__ int cost_of(const Span& s) { return max(s.n, 1) + OVER; }
 
 __device__ __forceinline__ void seq_sizes(const AttnArgs& a, int b, int& cu0, int& r, int& len) {
     cu0 = min(max(a.s.cu[b], 0), a.rows);
@@ -64,15 +67,34 @@ struct Shares {
     }
 };
 
-// Where a share stands on the line: a row block (b, h, rb), its keys, the line's position of its first unit.  Every method
-// is called by whole warps, all lanes alike.
-template <int ROWS, int UNIT>
+// Where a share stands on the line: a row block (b, h, rb), its keys, the line's position where it begins.  Every method is
+// called by whole warps, all lanes alike.
+template <int ROWS, int UNIT, int OVER>
 struct Cursor {
     int b, h, rb, cu0, r, len;
     Span s;
     long long begin;
-    __device__ __forceinline__ int cost() const { return cost_of(s); }
-    __device__ __forceinline__ long long end() const { return begin + cost_of(s); }
+    __device__ __forceinline__ int cost() const { return cost_of<OVER>(s); }
+    __device__ __forceinline__ long long end() const { return begin + cost(); }
+    // the units of the block before the line's position `at`.  With OVER a block of under four units is not cut, and no cut
+    // leaves one side without a unit; shares of four or more then have one unit at least of every block cut twice.
+    __device__ __forceinline__ int cut(long long at) const {
+        if (at <= begin) return 0;
+        if (at >= end()) return s.n;
+        const int rel = (int)(at - begin);
+        if (OVER == 0) return min(rel, s.n);
+        if (s.n < 4) return 2 * rel < cost() ? 0 : s.n;
+        return min(max((int)((long long)rel * s.n / cost()), 1), s.n - 1);
+    }
+    // this share's part of the block
+    __device__ __forceinline__ int from(long long share_begin) const { return cut(share_begin); }
+    __device__ __forceinline__ int to(long long share_end) const { return cut(share_end); }
+    // the share that holds the block's last unit, given one that holds an earlier one
+    __device__ __forceinline__ int last_share(const Shares& split, int share) const {
+        int k = split.of(end() - 1);
+        while (k > share && cut(split.start(k)) == s.n) k--;
+        return k;
+    }
     __device__ __forceinline__ bool block(const AttnArgs& a, int nrb) {
         return rb < nrb && row_block<ROWS, UNIT>(r, len, rb, a.group, a.window, s);
     }
@@ -124,7 +146,7 @@ struct Cursor {
 
 // The line's units in all and, once a share's start is known, the cursor at it: a block-wide exclusive sum over the
 // sequences, THREADS at a time.
-template <int ROWS, int UNIT, int THREADS>
+template <int ROWS, int UNIT, int OVER, int THREADS>
 struct Scan {
     struct Shared {
         long long warp_sum[THREADS / 32], units[THREADS], start[2];   // start: units before the share's first sequence, a head's
@@ -145,14 +167,14 @@ struct Scan {
         Span s;
         if (nrb <= 4) {
             if (b < a.s.batch)
-                for (int rb = 0; rb < nrb && row_block<ROWS, UNIT>(r, len, rb, a.group, a.window, s); rb++) units += cost_of(s);
+                for (int rb = 0; rb < nrb && row_block<ROWS, UNIT>(r, len, rb, a.group, a.window, s); rb++) units += cost_of<OVER>(s);
         } else {   // a warp a sequence, a lane a block
             __syncthreads();
             for (int i = warp; i < THREADS && b0 + i < a.s.batch; i += THREADS / 32) {
                 int c0, ri, li;
                 seq_sizes(a, b0 + i, c0, ri, li);
                 long long u = 0;
-                for (int rb = lane; rb < nrb && row_block<ROWS, UNIT>(ri, li, rb, a.group, a.window, s); rb += 32) u += cost_of(s);
+                for (int rb = lane; rb < nrb && row_block<ROWS, UNIT>(ri, li, rb, a.group, a.window, s); rb += 32) u += cost_of<OVER>(s);
 #pragma unroll
                 for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(~0u, u, o);
                 if (lane == 0) sh.units[i] = u;
@@ -182,7 +204,7 @@ struct Scan {
         return carry;
     }
     // after total(); ends with the block in step
-    __device__ __forceinline__ Cursor<ROWS, UNIT> seek(const AttnArgs& a, long long at) {
+    __device__ __forceinline__ Cursor<ROWS, UNIT, OVER> seek(const AttnArgs& a, long long at) {
         long long carry = 0;
         for (int b0 = 0; b0 < a.s.batch; b0 += THREADS) {
             if (a.s.batch > THREADS) carry = round(a, b0, carry, nullptr);   // else the round just made holds it
@@ -192,7 +214,7 @@ struct Scan {
             }
         }
         __syncthreads();
-        Cursor<ROWS, UNIT> p;
+        Cursor<ROWS, UNIT, OVER> p;
         p.b = sh.seq[0]; p.cu0 = sh.seq[1]; p.r = sh.seq[2]; p.len = sh.seq[3];
         p.seek(a, nrb, sh.start[0], sh.start[1], at);
         return p;
