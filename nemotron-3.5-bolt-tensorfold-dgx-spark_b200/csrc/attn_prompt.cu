@@ -116,7 +116,7 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
     bool dead = false;
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         if (warp == 9) {
             KvLoader<D, NS, At> kv{sk, sv, kfull, kempty, vfull, vempty, &mk, &mv, a};
             for (; !kv.dead;) {
@@ -146,9 +146,11 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                 p.advance(a, nrb);
             }
         } else {
-            // ------------------------------------------------------------ MMA
+            // ------------------------------------------------------------ MMA.  Votes on waits that ran out cost 50 cycles each
+            // here, so there is one a piece; the piece is finished without further waiting.
             int o = 0, k = 0, pr[2] = {0, 0};   // steps, pieces, P tiles so far
-            for (; !dead;) {
+            auto await = [&](uint32_t bar, uint32_t parity) { dead = dead || !wait_for(bar, parity); };
+            while (!dead) {
                 const int from = p.cut(begin), to = p.cut(end);
                 if (to > from) {
                     int ja[2], jb[2];
@@ -161,9 +163,9 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                         }
                         __syncwarp();
                     };
-                    if (!wait_for(qfull, k & 1) || !wait_for(kfull + o % NS * 8, o / NS & 1)) dead = true;
-                    dead = __any_sync(~0u, dead);
-                    if (dead) break;
+                    await(qfull, k & 1);
+                    await(kfull + o % NS * 8, o / NS & 1);
+                    __syncwarp();
                     tc_fence_after();
 #pragma unroll
                     for (int t = 0; t < 2; t++)
@@ -173,20 +175,18 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                         if (from + 1 == to) umma_commit(qempty);
                     }
                     __syncwarp();
-                    for (int j = from; j < to && !dead; j++, o++) {
+                    for (int j = from; j < to; j++, o++) {
                         const int st = o % NS, sn = (o + 1) % NS;
-                        if (!wait_for(vfull + st * 8, o / NS & 1)) dead = true;
-                        dead = __any_sync(~0u, dead);
-                        if (dead) break;
+                        await(vfull + st * 8, o / NS & 1);
+                        __syncwarp();
                         clear_unseen<D>(sv + st * L::kBytes, (p.s.u0 + j) * kKeys, p.s);
 #pragma unroll
                         for (int t = 0; t < 2; t++) {
                             if (j >= ja[t] && j < jb[t]) {
 #pragma unroll
                                 for (int half = 0; half < 2; half++) {
-                                    if (!wait_for(pready + (t * 2 + half) * 8, pr[t] & 1)) dead = true;
-                                    dead = __any_sync(~0u, dead);
-                                    if (dead) break;
+                                    await(pready + (t * 2 + half) * 8, pr[t] & 1);
+                                    __syncwarp();
                                     tc_fence_after();
                                     if (elect_one()) {
                                         issue_values<D>(tmem + 256 + t * D, tmem + t * kTile + half * 32, sv + st * L::kBytes + half * 8192, 4,
@@ -195,19 +195,16 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                                     }
                                     __syncwarp();
                                 }
-                                if (dead) break;
                                 pr[t]++;
                             }
                             if (t == 1 && elect_one()) umma_commit(vempty + st * 8);
                             if (t == 0 && j + 1 < to) {
-                                if (!wait_for(kfull + sn * 8, (o + 1) / NS & 1)) dead = true;
-                                dead = __any_sync(~0u, dead);
-                                if (dead) break;
+                                await(kfull + sn * 8, (o + 1) / NS & 1);
+                                __syncwarp();
                                 tc_fence_after();
                             }
                             if (j + 1 >= ja[t] && j + 1 < jb[t]) scores(t, sn);
                         }
-                        if (dead) break;
                         if (j + 1 < to && elect_one()) {
                             umma_commit(kempty + sn * 8);
                             if (j + 2 == to) umma_commit(qempty);
@@ -216,6 +213,7 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                     }
                     k++;
                 }
+                dead = __any_sync(~0u, dead);
                 if (p.end() >= end) break;
                 p.advance(a, nrb);
             }
@@ -226,27 +224,37 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
         }
     } else {
         // ---------------------------------------------------------------- softmax: warpgroup t, thread = row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t ts = tmem + t * kTile + ((uint32_t)quarter << 21), to_ = tmem + 256 + t * D + ((uint32_t)quarter << 21);
         const uint32_t stage = sout + warp * 4096;
         const float c = a.c;
         const uint64_t c2 = pair(c, c);
         int ns = 0;   // steps of the tile so far
+        // between a piece's steps the cursor lies in shared memory: the scores take the registers
+        At* kept = (At*)(base + (sout - sq) + warp * 4096);
         for (;;) {
             const int from = p.cut(begin), to = p.cut(end);
             if (to > from || (p.s.n == 0 && p.begin >= begin)) {
-                int ja, jb;
-                tile_steps(p, t, from, to, ja, jb);
-                const int n = jb - ja, row0 = p.rb * kRows + t * kTile, rows = min(kTile, p.r * a.group - row0);   // may be <= 0
-                const int mrow = min(row, max(rows, 1) - 1), tok = (row0 + mrow) / a.group;   // rows that are none: like the last
-                const int pos = p.len - p.r + tok, w0 = __shfl_sync(~0u, pos, 0), w1 = __shfl_sync(~0u, pos, 31);
+                int n, key0, pos, w0, w1;
+                {
+                    int ja, jb;
+                    tile_steps(p, t, from, to, ja, jb);
+                    n = jb - ja;
+                    key0 = (p.s.u0 + ja) * kKeys;
+                    const int row0 = p.rb * kRows + t * kTile, rows = min(kTile, p.r * a.group - row0);   // may be <= 0
+                    const int mrow = min(row, max(rows, 1) - 1);   // rows that are none: like the last
+                    pos = p.len - p.r + (row0 + mrow) / a.group;
+                    w0 = __shfl_sync(~0u, pos, 0);
+                    w1 = __shfl_sync(~0u, pos, 31);
+                }
+                if (lane == 0) *kept = p;
+                __syncwarp();
                 float ref = -INFINITY, sum = 0.f;   // the reference, in powers of two
                 bool settled = false;               // every row of the warp has a reference
-                for (int i = 0; i < n; i++, ns++) {
-                    const int key0 = (p.s.u0 + ja + i) * kKeys;
-                    if (!dead && !wait_for(sfull + t * 8, ns & 1)) dead = true;
-                    dead = __any_sync(~0u, dead);
+                for (int i = 0; i < n; i++, ns++, key0 += kKeys) {
+                    if (!dead && !wait_for(sfull + t * 8, ns & 1)) dead = true;   // goes on all the same: nobody waits for long
+                    __syncwarp();
                     tc_fence_after();
                     Scores s;
 #pragma unroll
@@ -262,7 +270,7 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                         settled = !__any_sync(~0u, ref == -INFINITY);
                         if (i > 0) {
                             if (!dead && !wait_for(odone + t * 8, ns - 1 & 1)) dead = true;
-                            dead = __any_sync(~0u, dead);
+                            __syncwarp();
                             tc_fence_after();
                             rescale<D>(to_, f);
                         }
@@ -271,38 +279,30 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                     const uint64_t z2 = pair(-z, -z);
                     uint64_t acc[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
                     auto hand_over = [&](int half) {   // half of P: its product may begin
-                        tmem_st_wait();
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) tc_mbar_arrive(pready + (t * 2 + half) * 8);
                     };
-                    if (part || !settled) {
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            probabilities<true>(s[j], c2, z2, acc, ts + j * 16);
-                            if (j & 1) hand_over(j / 2);
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            probabilities<false>(s[j], c2, z2, acc, ts + j * 16);
-                            if (j & 1) hand_over(j / 2);
-                        }
-                    }
+                    if (part || !settled) row_probabilities<true>(s, c2, z2, acc, ts, hand_over);
+                    else row_probabilities<false>(s, c2, z2, acc, ts, hand_over);
                     float s0, s1;
                     unpair(add2(acc[0], acc[1]), s0, s1);
                     sum += s0 + s1;
                 }
                 // ------------------------------------------------------------ out
-                if (n > 0) {
-                    if (!dead && !wait_for(odone + t * 8, ns - 1 & 1)) dead = true;
-                    dead = __any_sync(~0u, dead);
-                    tc_fence_after();
-                }
+                p = *kept;
+                __syncwarp();
                 const bool whole = from == 0 && to == p.s.n;
+                const int row0 = p.rb * kRows + t * kTile, rows = min(kTile, p.r * a.group - row0);
+                const int mrow = min(row, max(rows, 1) - 1), tok = (row0 + mrow) / a.group;
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;   // no key seen: zeros
                 const long long place = (p.cu0 + tok) * a.ldo + (int64_t)(p.h * a.group + row0 + mrow - tok * a.group) * D;
                 float* slot = slots(a.ws) + ((size_t)share * 2 + (from == 0 ? 1 : 0)) * kSlot<D, kRows>;
+                if (n > 0) {
+                    if (!dead && !wait_for(odone + t * 8, ns - 1 & 1)) dead = true;
+                    __syncwarp();
+                    tc_fence_after();
+                }
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 64) {   // 64 columns at a time
                     uint32_t v[2][32];
@@ -358,7 +358,7 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
             p.advance(a, nrb);
         }
     }
-    if (dead && lane == 0) atomicOr(&g_prompt_error, 1);
+    if (__any_sync(~0u, dead) && lane == 0) atomicOr(&g_prompt_error, 1);
     tc_fence_before();
     __syncthreads();
     if (warp == 8) {

@@ -217,11 +217,10 @@ __device__ __forceinline__ float row_top(const Scores& s) {   // NaN if any is
 // score makes its row NaN, by the reference, since ex2_poly does not carry NaN.
 __device__ __forceinline__ bool over_reference(float top, float ref) { return !(top <= ref + 8.f); }
 __device__ __forceinline__ float raised(float top, float ref) { return !over_reference(top, ref) ? ref : top < INFINITY ? top : NAN; }
-// probabilities of 32 keys by reference z, summed in fp32 and rounded to bf16, to TMEM; all: a key that is not seen counts
-// nothing at all, so none by ex2_poly
+// Probabilities of 32 keys by reference z, summed in fp32 and rounded to bf16; all: a key that is not seen counts nothing at
+// all, so none by ex2_poly
 template <bool ALL>
-__device__ __forceinline__ void probabilities(const uint32_t (&s)[32], uint64_t c2, uint64_t z2, uint64_t (&acc)[2], uint32_t tmem_p) {
-    uint32_t v[16];
+__device__ __forceinline__ void probabilities(const uint32_t (&s)[32], uint64_t c2, uint64_t z2, uint64_t (&acc)[2], uint32_t (&p)[16]) {
 #pragma unroll
     for (int y = 0; y < 16; y++) {
         const uint64_t e = fma2(pair(val(s[2 * y]), val(s[2 * y + 1])), c2, z2);
@@ -232,9 +231,25 @@ __device__ __forceinline__ void probabilities(const uint32_t (&s)[32], uint64_t 
             e1 = ex2(e1);
         } else ex2_poly(e, e0, e1);
         acc[y & 1] = add2(acc[y & 1], pair(e0, e1));
-        v[y] = pack_bf16(e0, e1);
+        p[y] = pack_bf16(e0, e1);
     }
-    tmem_st16(tmem_p, v);
+}
+// Those of the row's 128 keys to TMEM, 16 columns for 32 keys.  half(0) is called once the first 64 keys' have arrived there,
+// in the shadow of the third quarter's exponentials; half(1) at the end.
+template <bool ALL, typename F>
+__device__ __forceinline__ void row_probabilities(const Scores& s, uint64_t c2, uint64_t z2, uint64_t (&acc)[2], uint32_t tmem_p, F half) {
+    uint32_t p[16];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        probabilities<ALL>(s[j], c2, z2, acc, p);
+        if (j == 2) {
+            tmem_st_wait();
+            half(0);
+        }
+        tmem_st16(tmem_p + j * 16, p);
+    }
+    tmem_st_wait();
+    half(1);
 }
 // O of the row, D columns, times f
 template <int D>
