@@ -17,11 +17,17 @@ struct AttnArgs {
     KvSeqs s;
     int rows, max_rows;        // rows of q; the most rows of a sequence
     int hkv, group;            // kv heads, query heads a kv head
+    uint32_t group_mul, group_shift;
     int pages, page_log2;
     float c;                   // a score times c is the exponent in powers of two (log2 e * scale; softcap: log2 e * cap)
     float cap_in;              // softcap: scale / cap, 0: none
+    float cap_near;            // scores up to here in size are capped by cap_poly: s sum_k cap_poly[k] s^2k (attn_tc.cuh)
+    float cap_poly[3];
     int window;                // keys a row sees at most (INT_MAX / 2: no window)
     void* ws;
+    // row / group for rows below 2^31: with 2^s >= group > 2^(s-1) and mul = floor(2^32 (2^s - group) / group) + 1, the quotient
+    // is (floor(row mul / 2^32) + row) >> s (Granlund and Montgomery)
+    __device__ __forceinline__ int token(int row) const { return (int)((__umulhi((uint32_t)row, group_mul) + (uint32_t)row) >> group_shift); }
 };
 
 // The exponent of a raw score q . k: with a cap, cap * tanh(scale q.k / cap) = cap * (1 - 2 / (exp(2 y) + 1)).  The
@@ -68,18 +74,34 @@ inline bool attn_ok(const b200q_paged* kv, const void* q, int64_t ldq, int rows,
     return kv_ok(kv) && q && out && workspace && aligned(q, 16) && aligned(out, 16) && aligned(workspace, 16) && ldq % 8 == 0 &&
            ldo % 8 == 0 && rows >= 0 && hq > 0 && hq <= 4096 && hq % kv->hkv == 0 && ldq >= (int64_t)hq * kv->d &&
            ldo >= (int64_t)hq * kv->d && max_rows > 0 && (int64_t)max_rows * (hq / kv->hkv) < (1 << 30) && scale > 0.f &&
-           scale < INFINITY && softcap >= 0.f && softcap < INFINITY && window >= 0;
+           scale < INFINITY && softcap >= 0.f && softcap < 1e38f && (softcap == 0.f || scale / softcap < INFINITY) && window >= 0;
 }
 inline AttnArgs attn_args(const b200q_paged& kv, const void* q, int64_t ldq, int rows, int hq, int max_rows, float scale, float softcap,
                           int window, void* out, int64_t ldo, void* ws) {
     AttnArgs a = {};
     a.q = (const __nv_bfloat16*)q; a.ldq = ldq; a.rows = rows; a.out = (__nv_bfloat16*)out; a.ldo = ldo; a.s = kv_seqs(kv);
-    a.max_rows = max_rows; a.hkv = kv.hkv; a.group = hq / kv.hkv; a.pages = kv.pages; a.page_log2 = log2_of(kv.page);
+    a.max_rows = max_rows; a.hkv = kv.hkv; a.group = hq / kv.hkv;
+    while ((1u << a.group_shift) < (uint32_t)a.group) a.group_shift++;
+    a.group_mul = (uint32_t)((((uint64_t)((1u << a.group_shift) - a.group)) << 32) / a.group + 1);
+    a.pages = kv.pages; a.page_log2 = log2_of(kv.page);
     a.c = 1.4426950408889634f * (softcap > 0.f ? softcap : scale);
     a.cap_in = softcap > 0.f ? scale / softcap : 0.f;
+    // tanh(u) for |u| <= 3/8: u times the polynomial of degree 2 in u^2 with the least relative error (4.3e-6, a Remez fit), in
+    // terms of the score; its powers are ordinary numbers for scale / cap within 2^20 of 1
+    static const double tanh_poly[3] = {0.999995707885, -0.332780666598, 0.122647585951};
+    if (a.cap_in > 0x1p-20f && a.cap_in < 0x1p20f) {
+        a.cap_near = 0.375f / a.cap_in;
+        double u = a.cap_in;
+        for (int k = 0; k < 3; k++, u *= (double)a.cap_in * a.cap_in) a.cap_poly[k] = (float)(tanh_poly[k] * u);
+    }
     a.window = window > 0 && window < INT_MAX / 2 ? window : INT_MAX / 2;
     a.ws = ws;
     return a;
 }
+
+// The tensor-core form (attn_prompt.cu), which the decode form calls for more rows than its own kernel takes: workspace bytes
+// for up to `rows` rows a sequence and kv head, and the launch, returning a status.
+size_t prompt_workspace(int d, int64_t rows);
+int prompt_launch(const b200q_paged& kv, const AttnArgs& a, void* stream);
 
 }  // namespace b200q

@@ -4,8 +4,8 @@
 //
 // Bound by HBM: every key and value a row sees is read once for all rows and query heads of its kv head.
 //
-// Work is shared as attn_line.cuh says, in units of 16 keys (within one page, since pages hold 16 or more) and row blocks
-// of 8 NT rows, a CTA an SM.
+// Work is shared as attn_line.cuh says, in units of 16 keys (within one page, since pages hold 16 or more) and one row block
+// of 8 NT rows a kv head, a CTA an SM.  More than 16 rows a kv head are the tensor core's (attn_prompt.cu).
 //
 // A CTA is one producer warp, which walks the share and fills a ring of units by TMA (128-byte swizzle), and eight
 // consumer warps, which take the ring's units in turn.  Scores are formed transposed, S^T = K Q^T: 16 keys are the rows of
@@ -199,7 +199,7 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
             const int l = i & 31, nt = (i >> 5) % NT, kk = (i >> 5) / NT, row = nt * 8 + (l >> 2);
             uint2 v = make_uint2(0, 0);
             if (row < rows) {
-                const int rr = row0 + row, tok = rr / a.group;
+                const int rr = row0 + row, tok = a.token(rr);
                 const uint32_t* src = (const uint32_t*)(a.q + (p.cu0 + tok) * a.ldq + (int64_t)(p.h * a.group + rr - tok * a.group) * D +
                                                         kk * 16 + (l & 3) * 2);
                 v = make_uint2(src[0], src[4]);
@@ -207,18 +207,16 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
             qs[i] = v;
         }
         consumers_sync();
-        uint2 qr[NT <= 2 ? D / 16 * NT : 1];
-        if (NT <= 2) {
+        uint2 qr[D / 16 * NT];
 #pragma unroll
-            for (int i = 0; i < D / 16 * NT; i++) qr[i < (NT <= 2 ? D / 16 * NT : 1) ? i : 0] = qs[i * 32 + lane];
-        }
+        for (int i = 0; i < D / 16 * NT; i++) qr[i] = qs[i * 32 + lane];
         int place[NT][2];   // positions of this lane's columns (rows 8 nt + 2 t, + 1); none: before every key
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int row = nt * 8 + t * 2 + j;
-                place[nt][j] = row < rows ? p.len - p.r + (row0 + row) / a.group : -1;
+                place[nt][j] = row < rows ? p.len - p.r + a.token(row0 + row) : -1;
             }
         float m[NT][2], sum[NT][2], o[D / 16][NT][4];
 #pragma unroll
@@ -259,7 +257,7 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
                 ldsm4(k4, kt + (ch >> 3) * (kUnit * 128) + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4));
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    const uint2 b = NT <= 2 ? qr[NT <= 2 ? kk * NT + nt : 0] : qs[(kk * NT + nt) * 32 + lane];
+                    const uint2 b = qr[kk * NT + nt];
                     mma(s[nt], k4, b.x, b.y);
                 }
             }
@@ -374,7 +372,7 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
                     const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;   // no key seen: zeros
                     const uint32_t lo = transpose8(pack_bf16(v.x * i0, v.y * i1)), hi = transpose8(pack_bf16(v.z * i0, v.w * i1));
                     if (r0 + g < rows) {
-                        const int rr = row0 + r0 + g, tok = rr / a.group;
+                        const int rr = row0 + r0 + g, tok = a.token(rr);
                         uint32_t* dst = (uint32_t*)(a.out + (p.cu0 + tok) * a.ldo +
                                                     (int64_t)(p.h * a.group + rr - tok * a.group) * D + d0 + t * 2);
                         dst[0] = lo;
@@ -416,11 +414,17 @@ cudaError_t launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const Attn
     return launch(join_k<D, Shape<D, NT>::kRows>, dim3(ctas), dim3(256), 0, s, a);
 }
 
-int row_tiles(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+// Rows a kv head that this kernel takes.  From 17 on its accumulators are short of registers, and its S and PV products pay
+// for every eight rows; the tensor-core kernel's step costs the same up to 128.  32 query heads of d 128 over 4 kv heads, this
+// kernel (with 32 rows a block, as measured) against that: 32 sequences of 4096 keys, 2 rows each: 72 / 76 us; 3 rows: 145 / 76;
+// 16 rows: 477 / 86.  One of 512 keys: 16 / 26, 27 / 25, 33 / 35; d 64: 14 / 22, 18 / 22, 22 / 27.
+constexpr int kMostRows = 16;
+bool few(int hq, int hkv, int max_rows) { return (int64_t)max_rows * (hq / hkv) <= kMostRows; }
+int row_tiles(int hq, int hkv, int max_rows) { return max_rows * (hq / hkv) <= 8 ? 1 : 2; }
 
 size_t attend_ws(int hq, int hkv, int d, int max_rows) {
-    const int64_t rows = (int64_t)max_rows * (hq / hkv);
-    return kMaxShares * (sizeof(Desc) + 2 * (size_t)row_tiles(rows) * 8 * (d + 2) * sizeof(float));
+    if (!few(hq, hkv, max_rows)) return prompt_workspace(d, (int64_t)max_rows * (hq / hkv));
+    return kMaxShares * (sizeof(Desc) + 2 * (size_t)row_tiles(hq, hkv, max_rows) * 8 * (d + 2) * sizeof(float));
 }
 
 }  // namespace
@@ -441,15 +445,16 @@ int b200q_attn_decode(const b200q_paged* kv, const void* q, int64_t ldq, int row
     if (workspace_bytes < attend_ws(hq, kv->hkv, d, max_rows)) return B200Q_ENOSPACE;
     if (rows == 0) return B200Q_OK;
     const AttnArgs a = attn_args(*kv, q, ldq, rows, hq, max_rows, scale, softcap, window, out, ldo, workspace);
+    if (!few(hq, kv->hkv, max_rows)) return prompt_launch(*kv, a, stream);
     CUtensorMap mk, mv;
     if (!kv_tensor_map(&mk, kv->k_pages, kv->k_stride, *kv, kUnit, d / 64) ||
         !kv_tensor_map(&mv, kv->v_pages, kv->v_stride, *kv, kUnit, d / 64))
         return status_from(cudaErrorInvalidValue);
     const cudaStream_t s = (cudaStream_t)stream;
-    const int nt = row_tiles((int64_t)max_rows * a.group);
+    const bool one = row_tiles(hq, kv->hkv, max_rows) == 1;
     cudaError_t e;
-    if (d == 128) e = nt == 1 ? launch_rows<128, 1>(mk, mv, a, s) : nt == 2 ? launch_rows<128, 2>(mk, mv, a, s) : launch_rows<128, 4>(mk, mv, a, s);
-    else e = nt == 1 ? launch_rows<64, 1>(mk, mv, a, s) : nt == 2 ? launch_rows<64, 2>(mk, mv, a, s) : launch_rows<64, 4>(mk, mv, a, s);
+    if (d == 128) e = one ? launch_rows<128, 1>(mk, mv, a, s) : launch_rows<128, 2>(mk, mv, a, s);
+    else e = one ? launch_rows<64, 1>(mk, mv, a, s) : launch_rows<64, 2>(mk, mv, a, s);
     return status_from(e);
 }
 

@@ -28,14 +28,14 @@ struct Span {
     int u0, n, lo, hi, p0, p1;   // keys lo .. hi - 1; positions of its first and last row
 };
 template <int ROWS, int UNIT>
-__device__ __forceinline__ bool row_block(int r, int len, int rb, int group, int window, Span& s) {
-    const int first = rb * ROWS, all = r * group;
+__device__ __forceinline__ bool row_block(const AttnArgs& a, int r, int len, int rb, Span& s) {
+    const int first = rb * ROWS, all = r * a.group;
     if (first >= all) return false;
     const int last = min(first + ROWS, all) - 1;
-    s.p0 = len - r + first / group;
-    s.p1 = len - r + last / group;
+    s.p0 = len - r + a.token(first);
+    s.p1 = len - r + a.token(last);
     s.hi = max(s.p1 + 1, 0);
-    s.lo = min(max(0, s.p0 - window + 1), s.hi);
+    s.lo = min(max(0, s.p0 - a.window + 1), s.hi);
     s.u0 = s.lo / UNIT;
     s.n = s.hi > s.lo ? (s.hi + UNIT - 1) / UNIT - s.u0 : 0;
     return true;
@@ -84,7 +84,8 @@ struct Cursor {
         const int rel = (int)(at - begin);
         if (OVER == 0) return min(rel, s.n);
         if (s.n < 4) return 2 * rel < cost() ? 0 : s.n;
-        return min(max((int)((long long)rel * s.n / cost()), 1), s.n - 1);
+        const long long part = (long long)rel * s.n;
+        return min(max((int)(part < (1ll << 32) ? (unsigned)part / (unsigned)cost() : part / cost()), 1), s.n - 1);
     }
     // this share's part of the block
     __device__ __forceinline__ int from(long long share_begin) const { return cut(share_begin); }
@@ -96,7 +97,7 @@ struct Cursor {
         return k;
     }
     __device__ __forceinline__ bool block(const AttnArgs& a, int nrb) {
-        return rb < nrb && row_block<ROWS, UNIT>(r, len, rb, a.group, a.window, s);
+        return rb < nrb && row_block<ROWS, UNIT>(a, r, len, rb, s);
     }
     // to sequence b's block that holds the line's position `at`: b starts at `first`, each of its heads has a_head units
     __device__ __forceinline__ void seek(const AttnArgs& a, int nrb, long long first, long long a_head, long long at) {
@@ -167,14 +168,14 @@ struct Scan {
         Span s;
         if (nrb <= 4) {
             if (b < a.s.batch)
-                for (int rb = 0; rb < nrb && row_block<ROWS, UNIT>(r, len, rb, a.group, a.window, s); rb++) units += cost_of<OVER>(s);
+                for (int rb = 0; rb < nrb && row_block<ROWS, UNIT>(a, r, len, rb, s); rb++) units += cost_of<OVER>(s);
         } else {   // a warp a sequence, a lane a block
             __syncthreads();
             for (int i = warp; i < THREADS && b0 + i < a.s.batch; i += THREADS / 32) {
                 int c0, ri, li;
                 seq_sizes(a, b0 + i, c0, ri, li);
                 long long u = 0;
-                for (int rb = lane; rb < nrb && row_block<ROWS, UNIT>(ri, li, rb, a.group, a.window, s); rb += 32) u += cost_of<OVER>(s);
+                for (int rb = lane; rb < nrb && row_block<ROWS, UNIT>(a, ri, li, rb, s); rb += 32) u += cost_of<OVER>(s);
 #pragma unroll
                 for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(~0u, u, o);
                 if (lane == 0) sh.units[i] = u;
@@ -295,7 +296,7 @@ __global__ void __launch_bounds__(256, 4) join_k(AttnArgs a) {
         }
         if (live && mine == 0) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;   // no key seen: zeros
-            const int rr = d.row0 + r, tok = rr / a.group;
+            const int rr = d.row0 + r, tok = a.token(rr);
             uint32_t* dst = (uint32_t*)(a.out + (d.cu0 + tok) * a.ldo + (int64_t)(d.h * a.group + rr - tok * a.group) * D + lane * V);
 #pragma unroll
             for (int j = 0; j < V / 2; j++) dst[j] = pack_bf16(acc[2 * j] * inv, acc[2 * j + 1] * inv);

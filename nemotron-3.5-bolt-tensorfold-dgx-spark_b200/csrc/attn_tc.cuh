@@ -85,12 +85,6 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ bool done(uint32_t bar, uint32_t parity) {   // no waiting
-    uint32_t ok;
-    asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
-}
 // tc_mbar_wait, the first look without its suspend-time hint (15 cycles, not 50, where the phase is complete)
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
     uint32_t ok;
@@ -143,16 +137,6 @@ __device__ __forceinline__ void ex2_poly(uint64_t x, float& lo, float& hi) {
     lo = __uint_as_float(__float_as_uint(a) + (__float_as_uint(n0) << 23));
     hi = __uint_as_float(__float_as_uint(b) + (__float_as_uint(n1) << 23));
 }
-// tanh of two |u| <= 1: u times the polynomial of degree 5 in u^2 with the least relative error (6.2e-7, a Remez fit)
-__device__ __forceinline__ uint64_t tanh2_small(uint64_t u) {
-    const uint64_t v = mul2(u, u);
-    uint64_t p = fma2(pair(-0.003067060374f, -0.003067060374f), v, pair(0.01674311422f, 0.01674311422f));
-    p = fma2(p, v, pair(-0.05160567537f, -0.05160567537f));
-    p = fma2(p, v, pair(0.1328143328f, 0.1328143328f));
-    p = fma2(p, v, pair(-0.3332904279f, -0.3332904279f));
-    p = fma2(p, v, pair(0.999999404f, 0.999999404f));
-    return mul2(u, p);
-}
 
 // ---------------------------------------------------------------------------------------------------------
 // the scores of one row and 128 keys, bit patterns of fp32
@@ -160,36 +144,51 @@ __device__ __forceinline__ uint64_t tanh2_small(uint64_t u) {
 typedef uint32_t Scores[4][32];
 __device__ __forceinline__ float val(uint32_t x) { return __uint_as_float(x); }
 
-// s -> tanh(cap_in s); |cap_in s| <= 1 nearly always (a score below the cap): no special function then
-__device__ __forceinline__ void cap_scores(Scores& s, float cap_in) {
-    float far = 0.f;
+// s -> tanh(cap_in s): four packed operations two scores where all of the warp's lie below cap_near, as nearly always.
+// Otherwise the special functions, in TMEM and back: unrolled over the 128 scores beside the rest, the code alone cost a tenth
+// of a step that never ran it.
+__device__ __forceinline__ void cap_scores(Scores& s, uint32_t tmem_s, const AttnArgs& a) {
+    float m[4] = {};
+#pragma unroll
+    for (int y = 0; y < 32; y += 2)
+#pragma unroll
+        for (int j = 0; j < 4; j++) m[j] = max3(m[j], fabsf(val(s[j][y])), fabsf(val(s[j][y + 1])));
+    const float far = max3(max3(m[0], m[1], m[2]), m[3], m[3]);
+    if (__any_sync(~0u, !(far <= a.cap_near))) {
+#pragma unroll 1
+        for (int j = 0; j < 8; j++) {
+            uint32_t v[16];
+            tmem_ld16(tmem_s + j * 16, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int y = 0; y < 16; y++) v[y] = __float_as_uint(capped(val(v[y]), a.cap_in));
+            tmem_st16(tmem_s + j * 16, v);
+        }
+        tmem_st_wait();
+#pragma unroll
+        for (int j = 0; j < 4; j++) tmem_ld32(tmem_s + j * 32, s[j]);
+        tmem_ld_wait();
+        return;
+    }
+    uint64_t c[3];
+#pragma unroll
+    for (int k = 0; k < 3; k++) c[k] = pair(a.cap_poly[k], a.cap_poly[k]);
 #pragma unroll
     for (int j = 0; j < 4; j++)
 #pragma unroll
-        for (int y = 0; y < 32; y += 2) far = max3(far, fabsf(val(s[j][y])), fabsf(val(s[j][y + 1])));
-    if (__any_sync(~0u, !(far * cap_in <= 1.f))) {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int y = 0; y < 32; y++) s[j][y] = __float_as_uint(capped(val(s[j][y]), cap_in));
-    } else {
-        const uint64_t in2 = pair(cap_in, cap_in);
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int y = 0; y < 32; y += 2) {
-                float lo, hi;
-                unpair(tanh2_small(mul2(pair(val(s[j][y]), val(s[j][y + 1])), in2)), lo, hi);
-                s[j][y] = __float_as_uint(lo);
-                s[j][y + 1] = __float_as_uint(hi);
-            }
-    }
+        for (int y = 0; y < 32; y += 2) {
+            const uint64_t x = pair(val(s[j][y]), val(s[j][y + 1])), v = mul2(x, x);
+            float lo, hi;
+            unpair(mul2(x, fma2(fma2(c[2], v, c[1]), v, c[0])), lo, hi);
+            s[j][y] = __float_as_uint(lo);
+            s[j][y + 1] = __float_as_uint(hi);
+        }
 }
 // Keys key0 .. key0 + 127 that the row at `pos` does not see get no part (minus infinity).  w0, w1: the positions of the
-// warp's first and last row.  Returns whether some row of the warp does not see some key.
-__device__ __forceinline__ bool mask_scores(Scores& s, int key0, int pos, int w0, int w1, int window) {
+// warp's first and last row.
+__device__ __forceinline__ void mask_scores(Scores& s, int key0, int pos, int w0, int w1, int window) {
     const int all = w0 - key0, any = w1 - key0;   // columns up to which all rows, some row of the warp see
-    if (kKeys - 1 <= all && any - window < 0) return false;
+    if (kKeys - 1 <= all && any - window < 0) return;
     const int last = pos - key0, first = last - window;
     auto upto = [](int j) { return j >= 31 ? ~0u : j < 0 ? 0u : (2u << j) - 1; };   // bits 0 .. j
 #pragma unroll
@@ -199,7 +198,6 @@ __device__ __forceinline__ bool mask_scores(Scores& s, int key0, int pos, int w0
 #pragma unroll
             for (int y = 0; y < 32; y++) s[j][y] = seen & 1u << y ? s[j][y] : 0xff800000u;
         }
-    return true;
 }
 __device__ __forceinline__ float row_top(const Scores& s) {   // NaN if any is
     float m[4];
@@ -217,15 +215,14 @@ __device__ __forceinline__ float row_top(const Scores& s) {   // NaN if any is
 // score makes its row NaN, by the reference, since ex2_poly does not carry NaN.
 __device__ __forceinline__ bool over_reference(float top, float ref) { return !(top <= ref + 8.f); }
 __device__ __forceinline__ float raised(float top, float ref) { return !over_reference(top, ref) ? ref : top < INFINITY ? top : NAN; }
-// Probabilities of 32 keys by reference z, summed in fp32 and rounded to bf16; all: a key that is not seen counts nothing at
-// all, so none by ex2_poly
-template <bool ALL>
+// Probabilities of 32 keys by reference z, summed in fp32 and rounded to bf16.  A key that is not seen gets 2^-126 from
+// ex2_poly: nothing beside a row's sum, which is 2^-8 at least; a row that has seen no key yet drops it with its first reference.
 __device__ __forceinline__ void probabilities(const uint32_t (&s)[32], uint64_t c2, uint64_t z2, uint64_t (&acc)[2], uint32_t (&p)[16]) {
 #pragma unroll
     for (int y = 0; y < 16; y++) {
         const uint64_t e = fma2(pair(val(s[2 * y]), val(s[2 * y + 1])), c2, z2);
         float e0, e1;
-        if (ALL || y * kPoly % 8 < 8 - kPoly) {
+        if (y * kPoly % 8 < 8 - kPoly) {
             unpair(e, e0, e1);
             e0 = ex2(e0);
             e1 = ex2(e1);
@@ -236,12 +233,12 @@ __device__ __forceinline__ void probabilities(const uint32_t (&s)[32], uint64_t 
 }
 // Those of the row's 128 keys to TMEM, 16 columns for 32 keys.  half(0) is called once the first 64 keys' have arrived there,
 // in the shadow of the third quarter's exponentials; half(1) at the end.
-template <bool ALL, typename F>
+template <typename F>
 __device__ __forceinline__ void row_probabilities(const Scores& s, uint64_t c2, uint64_t z2, uint64_t (&acc)[2], uint32_t tmem_p, F half) {
     uint32_t p[16];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        probabilities<ALL>(s[j], c2, z2, acc, p);
+        probabilities(s[j], c2, z2, acc, p);
         if (j == 2) {
             tmem_st_wait();
             half(0);
@@ -345,7 +342,7 @@ __device__ __forceinline__ void load_q64(const AttnArgs& a, const At& p, int row
     long long place[2];   // of rows first + lane and + 32 in q
 #pragma unroll
     for (int y = 0; y < 2; y++) {
-        const int rr = row0 + first + y * 32 + lane, tok = rr / a.group;
+        const int rr = row0 + first + y * 32 + lane, tok = a.token(rr);
         place[y] = (p.cu0 + tok) * a.ldq + (int64_t)(p.h * a.group + rr - tok * a.group) * D;
     }
 #pragma unroll
