@@ -370,7 +370,7 @@ int b200q_kv_append(const b200q_paged* kv, const void* q, const void* k, const v
  * over the keys j of kv head h / (hq / hkv) with position - window < j <= position (window 0: all up to the position).
  * A row that sees no key gets zeros.  q [rows][hq][d] and out [rows][hq][d] bf16, rows ldq / ldo elements apart (multiples
  * of 8), 16-byte aligned, not overlapping.  Scores, sums and accumulators are fp32; the probabilities are rounded to bf16
- * for the product with v.  scale > 0, softcap >= 0 (0: none).
+ * for the product with v.  scale > 0; softcap 0 (none) to 1e38, scale / softcap finite.
  * decode: up to 16 rows a sequence (one new token, or a verify window).  prompt: any number.  max_rows >= the rows of
  * every sequence (a sequence with more sets bit 22 of b200q_device_error, and some of its rows are left out).
  * A table entry outside the cache reads as zeros, a length outside 0 .. width * page is brought inside; both set bit 21.

@@ -31,14 +31,16 @@ struct AttnArgs {
 };
 
 // The exponent of a raw score q . k: with a cap, cap * tanh(scale q.k / cap) = cap * (1 - 2 / (exp(2 y) + 1)).  The
-// subtraction leaves 2^-24 of the cap, far below bf16; tanh.approx (2^-11) would move a score of 50 by 0.02.
+// subtraction leaves 2^-23 of the cap, so below 2^-6 the series stands (its next term is 2^-26 of y); tanh.approx (2^-11)
+// would move a score of 50 by 0.02.
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ float capped(float x, float cap_in) {
-    return 1.f - __fdividef(2.f, ex2(x * cap_in * 2.885390081777927f) + 1.f);
+    const float y = x * cap_in, t = 1.f - __fdividef(2.f, ex2(y * 2.885390081777927f) + 1.f);
+    return fabsf(y) < 0.015625f ? fmaf(y * y * y, -1.f / 3.f, y) : t;
 }
 
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap* m) {

@@ -11,7 +11,7 @@
 // consumer warps, which take the ring's units in turn.  Scores are formed transposed, S^T = K Q^T: 16 keys are the rows of
 // an m16n8k16 and 8 query rows its columns, so a group of 4 or 8 query heads wastes half or none of it (16 x 8 the
 // other way round would waste three quarters).  The probabilities' accumulator becomes the B operand of O^T += V^T P^T by one
-// 8 x 8 transpose (movmatrix) each; P is rounded to bf16 there, V's type: 2^-9 relative on weights that are summed with
+// 8 x 8 transpose (movmatrix) each; P is rounded to bf16 there, V's type: 2^-8 at most on weights that are summed with
 // independent signs, below the output's own rounding.  m, the sum and O stay in fp32.
 #include "attn_line.cuh"
 #include "tcgen05.cuh"

@@ -77,7 +77,7 @@ struct Cursor {
     __device__ __forceinline__ int cost() const { return cost_of<OVER>(s); }
     __device__ __forceinline__ long long end() const { return begin + cost(); }
     // the units of the block before the line's position `at`.  With OVER a block of under four units is not cut, and no cut
-    // leaves one side without a unit; shares of four or more then have one unit at least of every block cut twice.
+    // leaves one side without a unit; shares of two or more then have one unit at least of every block cut twice.
     __device__ __forceinline__ int cut(long long at) const {
         if (at <= begin) return 0;
         if (at >= end()) return s.n;

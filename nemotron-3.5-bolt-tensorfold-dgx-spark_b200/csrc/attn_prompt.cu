@@ -42,7 +42,7 @@ template <bool NARROW>
 constexpr int kRows = NARROW ? kTile : 2 * kTile;
 constexpr int kThreads = 384;         // two softmax warpgroups; a MMA, a TMA and two Q warps
 constexpr int kOver = 2;              // what a row block costs besides its steps, in steps: its first and last step's waits
-constexpr int kMinShare = 4;          // a share is not smaller
+constexpr int kMinShare = 1 + kOver;  // a share is not smaller, but for the division's rest: a block of one step (4: 77 tokens 16.8 us, not 13.3)
 
 template <int D>
 struct Lay {
