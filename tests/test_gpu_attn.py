@@ -237,3 +237,51 @@ def test_shares_longer_than_the_ring(d, page, hq, hkv, rows):
     g = torch.Generator().manual_seed(1)
     sizes = [(rows, int(torch.randint(2000, 6000, (), generator=g))) for _ in range(9)] + [(rows, 16), (rows, 9000)]
     run(Step(sizes, hq, hkv, d, page, junk=math.nan), b200q.attn_decode)
+
+
+@pytest.mark.parametrize("f", BOTH)
+@pytest.mark.parametrize("hq,hkv,rows", [(17, 1, 1), (12, 2, 3), (8, 1, 16), (64, 2, 4), (40, 1, 16)])
+@pytest.mark.parametrize("d,page,window", [(128, 64, 0), (64, 16, 0), (64, 128, 300), (128, 256, 129)])
+def test_rows_of_one_tile_and_past_it(f, hq, hkv, rows, d, page, window):
+    """17 to 128 rows a kv head, and 640: one to 47 steps, an odd one at the end, blocks that shares cut and whole ones"""
+    sizes = [(rows, 128), (rows, 6000), (0, 9), (1, 129), (rows, rows), (rows, 257), (rows, 1500)]
+    run(Step(sizes, hq, hkv, d, page, pad=2, junk=math.nan), f, window=window)
+
+
+def test_more_row_blocks_than_a_warp_has_lanes():
+    """600 rows of 16 query heads: 38 blocks of 256 rows, shares that begin and end inside them"""
+    run(Step([(20, 20), (600, 700), (1, 3), (530, 530)], 16, 1, 64, 16, junk=math.nan), b200q.attn_prompt)
+    run(Step([(600, 700), (9, 5)], 16, 1, 128, 64), b200q.attn_prompt, window=40)
+
+
+@pytest.mark.parametrize("f", BOTH)
+@pytest.mark.parametrize("hq", [2, 20])
+@pytest.mark.parametrize("softcap", [0.5, 2.0, 30.0, 1e4, 1e7])
+def test_scores_on_all_sides_of_the_cap(f, hq, softcap):
+    """from scores far beyond the cap (there tanh's slope brings the scores' own errors to nothing) to caps far beyond the
+    scores: tanh is right to 2^-16 of its value throughout, so a probability to 2^-16 times 30, below the 2^-11 above"""
+    step = Step([(3, 500), (1, 129), (5, 40)], hq, 1, 64, 16)
+    run(step, f, q=queries(step, scale=5.0), softcap=softcap)
+    step = Step([(3, 500), (1, 129), (5, 40)], hq, 1, 128, 32)
+    run(step, f, softcap=softcap, window=100)
+
+
+@pytest.mark.parametrize("f", BOTH)
+@pytest.mark.parametrize("hq", [2, 20])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_score_that_is_no_number_spoils_its_rows_alone(f, hq, bad):
+    """query heads 0 and the last hold it; the others are as the definition has them"""
+    step = Step([(2, 300), (1, 60)], hq, 1, 64, 16)
+    q = queries(step)
+    spoilt = q.clone()
+    spoilt[0, 0, 3] = spoilt[1, hq - 1, 3] = bad
+    for softcap in (0.0, 20.0):
+        want = attend(step, q, softcap=softcap)
+        step.to(DEV)
+        out = f(spoilt.to(DEV), *step.args(), 2, softcap=softcap).cpu().double()
+        left = torch.ones(3, hq, dtype=torch.bool)
+        left[0, 0] = left[1, hq - 1] = False
+        a = attend(Abs(step), q, softcap=softcap)
+        assert ((out - want).abs()[left] <= (2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -10 + 300 * 2.0 ** -24) * a)[left]).all()
+        if softcap == 0 or math.isnan(bad):
+            assert torch.isnan(out[0, 0]).all() and torch.isnan(out[1, hq - 1]).all()

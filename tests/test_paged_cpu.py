@@ -57,6 +57,24 @@ def test_attention_refuses(f, kw):
     assert call(f, ATTN, kw) == b200q.EINVAL
 
 
+@pytest.mark.parametrize("f", ["b200q_attn_decode", "b200q_attn_prompt"])
+@pytest.mark.parametrize("kw", [dict(softcap=1e-45), dict(softcap=2e38), dict(softcap=float("inf"))])
+def test_caps_out_of_range_are_refused(f, kw):
+    assert call(f, ATTN, kw) == b200q.EINVAL
+
+
+def test_workspace_follows_the_rows_a_kv_head():
+    """up to 8 and 16 rows a kv head, up to a tile of 128, more"""
+    w = b200q.lib().b200q_attn_decode_workspace_bytes
+    sizes = [w(8, 1, 128, 1), w(16, 1, 128, 1), w(17, 1, 128, 1), w(8, 1, 128, 16), w(9, 1, 128, 16), w(512, 1, 128, 16)]
+    assert sizes[0] < sizes[1] < sizes[2] == sizes[3] < sizes[4] == sizes[5]
+    p = b200q.lib().b200q_attn_prompt_workspace_bytes
+    assert p(8, 1, 128, 16, 16, 1) == sizes[3] and p(8, 1, 128, 17, 17, 1) == sizes[4]
+    for f, rows in (("b200q_attn_decode", 16), ("b200q_attn_prompt", 100)):   # one byte short
+        need = w(4, 2, 128, rows) if "decode" in f else p(4, 2, 128, rows, rows, 2)
+        assert call(f, ATTN, dict(max_rows=rows, wsb=need - 1)) == b200q.ENOSPACE
+
+
 def test_attention_of_no_rows_too_many_and_too_little_workspace():
     L = b200q.lib()
     for f in ("b200q_attn_decode", "b200q_attn_prompt"):
