@@ -684,16 +684,16 @@ def k_kv_append(q, k, v, k_pages, v_pages, table, lens, cu, inv_freq=None, inter
 
 
 @functools.lru_cache(maxsize=1024)
-def _attn_workspace(name, dev, *sizes):
-    with torch.cuda.device(dev):   # the prompt form's depends on the device's SMs
-        return max(getattr(lib(), f"b200q_{name}_workspace_bytes")(*sizes), 16)
+def _attn_workspace(name, *sizes):
+    return max(getattr(lib(), f"b200q_{name}_workspace_bytes")(*sizes), 16)
 
 
 def _attend(name, q, k_pages, v_pages, table, lens, cu, max_rows, scale, softcap, window, out):
     kv, dev, hkv, d, batch = _paged(k_pages, v_pages, table, lens, cu)
     rows, hq, ldq = _heads(q, "q", dev, torch.bfloat16, d)
     if out is None:
-        out = torch.empty(rows, hq, d, dtype=torch.bfloat16, device=k_pages.device)
+        # empty_like takes 0.5 us less on the host
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(rows, hq, d, dtype=torch.bfloat16, device=k_pages.device)
         ldo = hq * d
     else:
         no, ho, ldo = _heads(out, "out", dev, torch.bfloat16, d)
@@ -703,9 +703,9 @@ def _attend(name, q, k_pages, v_pages, table, lens, cu, max_rows, scale, softcap
         return out
     L = lib()
     if name == "attn_decode":
-        fn, nb = L.b200q_attn_decode, _attn_workspace(name, dev, hq, hkv, d, max_rows)
+        fn, nb = L.b200q_attn_decode, _attn_workspace(name, hq, hkv, d, max_rows)
     else:
-        fn, nb = L.b200q_attn_prompt, _attn_workspace(name, dev, hq, hkv, d, rows, max_rows, batch)
+        fn, nb = L.b200q_attn_prompt, _attn_workspace(name, hq, hkv, d, rows, max_rows, batch)
     # scratch of this call alone: calls on other streams, and captured ones, have their own
     ws = torch.empty(nb, dtype=torch.uint8, device=k_pages.device)
     st = _call(dev, fn, kv, q.data_ptr(), ldq, rows, hq, max_rows, d ** -0.5 if scale is None else scale, softcap, window,

@@ -191,6 +191,11 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
     for (long long at = begin; at < end;) {
         // units skip .. of the row block are this share's
         const int skip = p.from(begin), n = p.to(end) - skip, u0 = p.s.u0 + skip;
+        if (n == 0 && (p.s.n > 0 || p.begin < begin)) {   // a cut that left this share nothing of the block
+            at = p.end();
+            if (at < end) p.advance(a, nrb);
+            continue;
+        }
         const bool whole_block = n == p.s.n;
         const int row0 = p.rb * RB, rows = min(RB, p.r * a.group - row0);
         // Q in fragment order: fragment (kk, nt), lane (g, t): values 16 kk + 2 t, + 1 and + 8, + 9 of row 8 nt + g

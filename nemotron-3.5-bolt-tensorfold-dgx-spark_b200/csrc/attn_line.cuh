@@ -76,13 +76,15 @@ struct Cursor {
     long long begin;
     __device__ __forceinline__ int cost() const { return cost_of<OVER>(s); }
     __device__ __forceinline__ long long end() const { return begin + cost(); }
-    // the units of the block before the line's position `at`.  With OVER a block of under four units is not cut, and no cut
-    // leaves one side without a unit; shares of two or more then have one unit at least of every block cut twice.
+    // The units of the block before the line's position `at`.  Without OVER no cut leaves fewer than four units on a side, and
+    // shares have eight or more: a piece of its own costs 3900 cycles, eight units more 1250 (one sequence of 1000 keys, 15.75
+    // units a share: 9200 cycles, not 13400).  With OVER a block of under four units is not cut, and no cut leaves one side
+    // without a unit; shares of two or more then have one unit at least of every block cut twice.
     __device__ __forceinline__ int cut(long long at) const {
         if (at <= begin) return 0;
         if (at >= end()) return s.n;
         const int rel = (int)(at - begin);
-        if (OVER == 0) return min(rel, s.n);
+        if (OVER == 0) return s.n < 8 ? (2 * rel < s.n ? 0 : s.n) : rel < 4 ? 0 : rel > s.n - 4 ? s.n : rel;
         if (s.n < 4) return 2 * rel < cost() ? 0 : s.n;
         const long long part = (long long)rel * s.n;
         return min(max((int)(part < (1ll << 32) ? (unsigned)part / (unsigned)cost() : part / cost()), 1), s.n - 1);
@@ -145,8 +147,8 @@ struct Cursor {
     }
 };
 
-// The line's units in all and, once a share's start is known, the cursor at it: a block-wide exclusive sum over the
-// sequences, THREADS at a time.
+// The line's units in all and, once a share's start is known, the cursor at it: an exclusive sum over the sequences, by each
+// warp for itself where they are 32 or fewer (500 cycles less before the first load), else block-wide, THREADS at a time.
 template <int ROWS, int UNIT, int OVER, int THREADS>
 struct Scan {
     struct Shared {
@@ -154,12 +156,13 @@ struct Scan {
         int seq[4];                                                    // that sequence and its sizes
     };
     Shared& sh;
-    long long units, below;   // of sequence b0 + thread: those of a head, those of the sequences before
+    long long units, below;   // of sequence b0 + thread (each warp: b0 + lane): those of a head, those of the sequences before
     int cu0, r, len, nrb;
+    __device__ __forceinline__ bool alone(const AttnArgs& a) const { return a.s.batch <= 32 && nrb <= 4; }
     __device__ __forceinline__ Scan(Shared& shared, int nrb_) : sh(shared), units(0), below(0), cu0(0), r(0), len(0), nrb(nrb_) {}
 
     __device__ __forceinline__ long long round(const AttnArgs& a, int b0, long long carry, int* error) {
-        const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = b0 + tid;
+        const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = alone(a) ? lane : b0 + tid;
         units = 0;
         if (b < a.s.batch) {
             seq_sizes(a, b, cu0, r, len);
@@ -189,6 +192,10 @@ struct Scan {
             const long long v = __shfl_up_sync(~0u, sum, o);
             if (lane >= o) sum += v;
         }
+        if (alone(a)) {
+            below = sum - units * a.hkv;
+            return __shfl_sync(~0u, sum, 31);
+        }
         __syncthreads();   // the sums of the round before have been read
         if (lane == 31) sh.warp_sum[warp] = sum;
         __syncthreads();
@@ -204,9 +211,17 @@ struct Scan {
         for (int b0 = 0; b0 < a.s.batch; b0 += THREADS) carry = round(a, b0, carry, error);
         return carry;
     }
-    // after total(); ends with the block in step
+    // after total()
     __device__ __forceinline__ Cursor<ROWS, UNIT, OVER> seek(const AttnArgs& a, long long at) {
         long long carry = 0;
+        Cursor<ROWS, UNIT, OVER> p;
+        if (alone(a)) {
+            const int from = __ffs(__ballot_sync(~0u, units > 0 && below <= at && at < below + units * a.hkv)) - 1;
+            p.b = from;
+            p.cu0 = __shfl_sync(~0u, cu0, from); p.r = __shfl_sync(~0u, r, from); p.len = __shfl_sync(~0u, len, from);
+            p.seek(a, nrb, __shfl_sync(~0u, below, from), __shfl_sync(~0u, units, from), at);
+            return p;
+        }
         for (int b0 = 0; b0 < a.s.batch; b0 += THREADS) {
             if (a.s.batch > THREADS) carry = round(a, b0, carry, nullptr);   // else the round just made holds it
             if (units > 0 && below <= at && at < below + units * a.hkv) {
@@ -215,7 +230,6 @@ struct Scan {
             }
         }
         __syncthreads();
-        Cursor<ROWS, UNIT, OVER> p;
         p.b = sh.seq[0]; p.cu0 = sh.seq[1]; p.r = sh.seq[2]; p.len = sh.seq[3];
         p.seek(a, nrb, sh.start[0], sh.start[1], at);
         return p;
