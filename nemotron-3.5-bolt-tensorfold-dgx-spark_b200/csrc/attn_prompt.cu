@@ -303,7 +303,6 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                     unpair(add2(acc[0], acc[1]), s0, s1);
                     sum += s0 + s1;
                 }
-                if (ref == -INFINITY) sum = 0.f;
                 // ------------------------------------------------------------ out
                 p = *kept;
                 __syncwarp();

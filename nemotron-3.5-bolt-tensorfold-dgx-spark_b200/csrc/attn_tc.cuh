@@ -11,7 +11,6 @@ using line::pack_bf16;
 
 constexpr int kKeys = 128;   // keys of a step
 constexpr int kTile = 128;   // rows of a tile
-constexpr int kPoly = 2;     // of 8 pairs of exponentials, those by polynomial (0: 5 % slower at 8192 tokens; 3: 2 %)
 
 constexpr uint32_t kIdescBf16 = (1u << 4) | (1u << 7) | (1u << 10) | (128u >> 4) << 24;   // fp32 += bf16 bf16, M = 128
 constexpr uint32_t kIdescQK = kIdescBf16 | (128u >> 3) << 17;
@@ -119,24 +118,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {   // NaN if a
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// 2^x for two x <= 8, without the special-function unit: x = n + f, |f| <= 1/2, and 2^f by the polynomial of degree 3
-// with the least relative error there (7.5e-5 = 2^-13.7, a Remez fit; the result is rounded to bf16 next, 2^-8).  Below
-// 2^-126 it stays there.  Adding 1.5 2^23 leaves n in the low bits of the sum, and n << 23 adds to the exponent.
-__device__ __forceinline__ void ex2_poly(uint64_t x, float& lo, float& hi) {
-    const uint64_t magic = pair(12582912.f, 12582912.f);
-    float a, b;
-    unpair(x, a, b);
-    x = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
-    const uint64_t t = add2(x, magic), n = add2(t, pair(-12582912.f, -12582912.f)), f = fma2(n, pair(-1.f, -1.f), x);
-    uint64_t p = fma2(pair(0.05517166852951050f, 0.05517166852951050f), f, pair(0.24261112511157990f, 0.24261112511157990f));
-    p = fma2(p, f, pair(0.69326096773147583f, 0.69326096773147583f));
-    p = fma2(p, f, pair(0.99992805719375610f, 0.99992805719375610f));
-    float n0, n1;
-    unpair(t, n0, n1);
-    unpair(p, a, b);
-    lo = __uint_as_float(__float_as_uint(a) + (__float_as_uint(n0) << 23));
-    hi = __uint_as_float(__float_as_uint(b) + (__float_as_uint(n1) << 23));
-}
 
 // ---------------------------------------------------------------------------------------------------------
 // the scores of one row and 128 keys, bit patterns of fp32
@@ -212,21 +193,19 @@ __device__ __forceinline__ float row_top(const Scores& s) {   // NaN if any is
     return max3(max3(m[0], m[1], m[2]), m[3], m[3]);
 }
 // The reference after a step whose largest exponent is `top`: raised only when it is exceeded by 2^8.  An infinite or NaN
-// score makes its row NaN, by the reference, since ex2_poly does not carry NaN.
+// score makes its row NaN, by the reference.
 __device__ __forceinline__ bool over_reference(float top, float ref) { return !(top <= ref + 8.f); }
 __device__ __forceinline__ float raised(float top, float ref) { return !over_reference(top, ref) ? ref : top < INFINITY ? top : NAN; }
-// Probabilities of 32 keys by reference z, summed in fp32 and rounded to bf16.  A key that is not seen gets 2^-126 from
-// ex2_poly: nothing beside a row's sum, which is 2^-8 at least; a row that has seen no key yet drops it with its first reference.
+// Probabilities of 32 keys by reference z, summed in fp32 and rounded to bf16.  All by the special-function unit: a quarter of
+// them by a polynomial of degree 3 relieves it, but the other pipes and the code's length gave up more (8192 tokens 490 us with
+// it, 480 without; ragged prompts 81 / 78).
 __device__ __forceinline__ void probabilities(const uint32_t (&s)[32], uint64_t c2, uint64_t z2, uint64_t (&acc)[2], uint32_t (&p)[16]) {
 #pragma unroll
     for (int y = 0; y < 16; y++) {
-        const uint64_t e = fma2(pair(val(s[2 * y]), val(s[2 * y + 1])), c2, z2);
         float e0, e1;
-        if (y * kPoly % 8 < 8 - kPoly) {
-            unpair(e, e0, e1);
-            e0 = ex2(e0);
-            e1 = ex2(e1);
-        } else ex2_poly(e, e0, e1);
+        unpair(fma2(pair(val(s[2 * y]), val(s[2 * y + 1])), c2, z2), e0, e1);
+        e0 = ex2(e0);
+        e1 = ex2(e1);
         acc[y & 1] = add2(acc[y & 1], pair(e0, e1));
         p[y] = pack_bf16(e0, e1);
     }
