@@ -23,6 +23,7 @@ struct AttnArgs {
     float cap_in;              // softcap: scale / cap, 0: none
     float cap_near;            // scores up to here in size are capped by cap_poly: s sum_k cap_poly[k] s^2k (attn_tc.cuh)
     float cap_poly[3];
+    bool whole;                // decode form: no row block is cut, so none is joined
     int window;                // keys a row sees at most (INT_MAX / 2: no window)
     void* ws;
     // row / group for rows below 2^31: with 2^s >= group > 2^(s-1) and mul = floor(2^32 (2^s - group) / group) + 1, the quotient

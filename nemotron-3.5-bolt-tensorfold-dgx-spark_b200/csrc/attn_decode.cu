@@ -416,7 +416,7 @@ cudaError_t launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const Attn
     const int ctas = min(device_sms(), kMaxShares);
     e = launch(attn_rows_k<D, NT>, dim3(ctas), dim3((kWarps + 1) * 32), smem, s, mk, mv, a);
     if (e != cudaSuccess) return e;
-    return launch(join_k<D, Shape<D, NT>::kRows>, dim3(ctas), dim3(256), 0, s, a);
+    return a.whole ? e : launch(join_k<D, Shape<D, NT>::kRows>, dim3(ctas), dim3(256), 0, s, a);
 }
 
 // Rows a kv head that this kernel takes.  From 17 on its accumulators are short of registers, and its S and PV products pay
@@ -424,6 +424,11 @@ cudaError_t launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const Attn
 // kernel (with 32 rows a block, as measured) against that: 32 sequences of 4096 keys, 2 rows each: 72 / 76 us; 3 rows: 145 / 76;
 // 16 rows: 477 / 86.  One of 512 keys: 16 / 26, 27 / 25, 33 / 35; d 64: 14 / 22, 18 / 22, 22 / 27.
 constexpr int kMostRows = 16;
+// Where the page table holds no more keys a sequence, and there is a CTA for every block, blocks are not cut: a CTA then reads a
+// block's keys alone, but nothing is joined and the second launch is saved.  In a stream of calls, whole against cut, 32 heads of
+// d 128 over 8, one sequence: 500 keys 7.2 / 8.5 us, 1000 keys 10.3 / 10.0; 16 sequences: 9.1 / 13.2 and 15.4 / 20.1.  The host's
+// part of a call is 13.3 / 15.8.
+constexpr int kWholeKeys = 1024;
 bool few(int hq, int hkv, int max_rows) { return (int64_t)max_rows * (hq / hkv) <= kMostRows; }
 int row_tiles(int hq, int hkv, int max_rows) { return max_rows * (hq / hkv) <= 8 ? 1 : 2; }
 
@@ -449,8 +454,9 @@ int b200q_attn_decode(const b200q_paged* kv, const void* q, int64_t ldq, int row
     const int d = kv->d;
     if (workspace_bytes < attend_ws(hq, kv->hkv, d, max_rows)) return B200Q_ENOSPACE;
     if (rows == 0) return B200Q_OK;
-    const AttnArgs a = attn_args(*kv, q, ldq, rows, hq, max_rows, scale, softcap, window, out, ldo, workspace);
+    AttnArgs a = attn_args(*kv, q, ldq, rows, hq, max_rows, scale, softcap, window, out, ldo, workspace);
     if (!few(hq, kv->hkv, max_rows)) return prompt_launch(*kv, a, stream);
+    a.whole = (int64_t)kv->width * kv->page <= kWholeKeys && (int64_t)kv->batch * kv->hkv <= min(device_sms(), kMaxShares);
     CUtensorMap mk, mv;
     if (!kv_tensor_map(&mk, kv->k_pages, kv->k_stride, *kv, kUnit, d / 64) ||
         !kv_tensor_map(&mv, kv->v_pages, kv->v_stride, *kv, kUnit, d / 64))

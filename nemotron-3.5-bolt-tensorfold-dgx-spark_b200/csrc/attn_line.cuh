@@ -74,17 +74,18 @@ struct Cursor {
     int b, h, rb, cu0, r, len;
     Span s;
     long long begin;
+    bool whole;
     __device__ __forceinline__ int cost() const { return cost_of<OVER>(s); }
     __device__ __forceinline__ long long end() const { return begin + cost(); }
-    // The units of the block before the line's position `at`.  Without OVER no cut leaves fewer than four units on a side, and
-    // shares have eight or more: a piece of its own costs 3900 cycles, eight units more 1250 (one sequence of 1000 keys, 15.75
-    // units a share: 9200 cycles, not 13400).  With OVER a block of under four units is not cut, and no cut leaves one side
-    // without a unit; shares of two or more then have one unit at least of every block cut twice.
+    // The units of the block before the line's position `at`.  Whole: all or none.  Without OVER no cut leaves fewer than four
+    // units on a side, and shares have eight or more: a piece of its own costs 3900 cycles, eight units more 1250 (one sequence
+    // of 1000 keys, 15.75 units a share: 9200 cycles, not 13400).  With OVER a block of under four units is not cut, and no cut
+    // leaves one side without a unit; shares of two or more then have one unit at least of every block cut twice.
     __device__ __forceinline__ int cut(long long at) const {
         if (at <= begin) return 0;
         if (at >= end()) return s.n;
         const int rel = (int)(at - begin);
-        if (OVER == 0) return s.n < 8 ? (2 * rel < s.n ? 0 : s.n) : rel < 4 ? 0 : rel > s.n - 4 ? s.n : rel;
+        if (OVER == 0) return s.n < 8 || whole ? (2 * rel < s.n ? 0 : s.n) : rel < 4 ? 0 : rel > s.n - 4 ? s.n : rel;
         if (s.n < 4) return 2 * rel < cost() ? 0 : s.n;
         const long long part = (long long)rel * s.n;
         return min(max((int)(part < (1ll << 32) ? (unsigned)part / (unsigned)cost() : part / cost()), 1), s.n - 1);
@@ -215,6 +216,7 @@ struct Scan {
     __device__ __forceinline__ Cursor<ROWS, UNIT, OVER> seek(const AttnArgs& a, long long at) {
         long long carry = 0;
         Cursor<ROWS, UNIT, OVER> p;
+        p.whole = a.whole;
         if (alone(a)) {
             const int from = __ffs(__ballot_sync(~0u, units > 0 && below <= at && at < below + units * a.hkv)) - 1;
             p.b = from;

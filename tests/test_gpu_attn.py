@@ -285,3 +285,15 @@ def test_a_score_that_is_no_number_spoils_its_rows_alone(f, hq, bad):
         assert ((out - want).abs()[left] <= (2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -10 + 300 * 2.0 ** -24) * a)[left]).all()
         if softcap == 0 or math.isnan(bad):
             assert torch.isnan(out[0, 0]).all() and torch.isnan(out[1, hq - 1]).all()
+
+
+@pytest.mark.parametrize("f", BOTH)
+@pytest.mark.parametrize("d,page,width", [(128, 64, 16), (128, 64, 17), (64, 16, 24), (64, 16, 25), (128, 128, 3)])
+@pytest.mark.parametrize("batch", [1, 18, 40])
+def test_tables_at_the_widths_that_leave_blocks_whole(f, d, page, width, batch):
+    """384 and 1024 keys of table a sequence, and a page more; more blocks than CTAs; windows that empty none and some"""
+    g = torch.Generator().manual_seed(2)
+    top = width * page
+    sizes = [(1, top)] + [(1, int(torch.randint(0, top + 1, (), generator=g))) for _ in range(batch - 1)]
+    run(Step(sizes, 8, 4, d, page, junk=math.nan), f)
+    run(Step([(3, n) for _, n in sizes], 8, 4, d, page, junk=math.nan), f, window=37)
