@@ -348,7 +348,7 @@ typedef struct b200q_paged {
     int width, batch;
 } b200q_paged;
 
-/* Append (the role of kv_store_k, bolt_kernels.cu:1735, with the steps before it): for each of `rows` rows
+/* Append (libbolt: bolt_kernels.cu:1735, and the steps before it): for each of `rows` rows
  *   q_out = bf16(rotate(norm(q))),  k_pages[slot] = bf16(rotate(norm(k))),  v_pages[slot] = bf16(v)
  * q [rows][hq][d], k and v [rows][hkv][d], fp32 or bf16 (x_dtype), rows ldq / ldk / ldv elements apart (16-byte
  * multiples; the fused projection's output can be passed as it is), q_out [rows][hq][d] bf16, rows ldo apart; q_out may
@@ -364,8 +364,8 @@ int b200q_kv_append(const b200q_paged* kv, const void* q, const void* k, const v
                     const void* q_norm, const void* k_norm, int norm_dtype, float eps, void* q_out, int64_t ldo,
                     void* stream);
 
-/* Attention over the cache (the roles of attn_part_k / attn_blk_part_k, bolt_kernels.cu:1779-2009, and attn_mma_part_k /
- * attn_mma2_part_k, bolt_mma.cu:1406-1724, with their combines): for each row of the step and query head h
+/* Attention over the cache (libbolt: bolt_kernels.cu:1779-2009, bolt_mma.cu:1406-1724): for each row of the step and
+ * query head h
  *   out = sum_j p_j v_j / sum_j p_j,   p_j = exp(s_j),   s_j = scale q . k_j, or softcap tanh(scale q . k_j / softcap)
  * over the keys j of kv head h / (hq / hkv) with position - window < j <= position (window 0: all up to the position).
  * A row that sees no key gets zeros.  q [rows][hq][d] and out [rows][hq][d] bf16, rows ldq / ldo elements apart (multiples

@@ -564,7 +564,7 @@ def moe_prompt(up, down, E, H, F, counts, offsets, order, topk, x, mo=None, act=
 
 
 # -------------------------------------------------------------------------------------------------------------
-# paged attention (kv_store and the attention between the q/k/v projection and o_proj)
+# paged attention (the cache and the attention between the q/k/v projection and o_proj)
 #
 # A decode step makes three of these calls a layer with a few microseconds of work each, so their checks read every tensor
 # attribute once.
@@ -639,7 +639,7 @@ def _call(dev, fn, *args):
 
 def k_kv_append(q, k, v, k_pages, v_pages, table, lens, cu, inv_freq=None, interleaved=False, q_norm=None, k_norm=None,
                 eps=1e-6, q_out=None):
-    """A step's keys and values into the paged cache (kv_store), norm and rotation on the way; see b200q_kv_append.
+    """A step's keys and values into the paged cache, norm and rotation on the way; see b200q_kv_append.
 
     q [rows][hq][d] (or None), k and v [rows][hkv][d]: fp32 or bf16, rows at any 16-byte pitch (views of the fused
     projection's output); k_pages / v_pages [pages][hkv][page][d] bf16; table [batch][width], lens [batch],

