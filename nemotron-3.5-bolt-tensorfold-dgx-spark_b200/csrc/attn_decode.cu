@@ -417,7 +417,7 @@ cudaError_t launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const Attn
     const int ctas = min(device_sms(), kMaxShares);
     e = launch(attn_rows_k<D, NT>, dim3(ctas), dim3((kWarps + 1) * 32), smem, s, mk, mv, a);
     if (e != cudaSuccess) return e;
-    return a.whole ? e : launch(join_k<D, Shape<D, NT>::kRows>, dim3(ctas), dim3(256), 0, s, a);
+    return a.whole ? e : launch(join_k<D, Shape<D, NT>::kRows>, dim3(ctas, NT), dim3(256), 0, s, a);
 }
 
 // Rows a kv head that this kernel takes.  From 17 on its accumulators are short of registers, and its S and PV products pay

@@ -448,7 +448,8 @@ cudaError_t launch_prompt(const b200q_paged& kv, const AttnArgs& a, cudaStream_t
     if (e != cudaSuccess) return e;
     // blocks of under four steps are not cut: nothing to join (77 tokens 12.6 -> 10.3 us)
     if ((int64_t)kv.width * kv.page <= 3 * kKeys) return e;
-    return launch(join_k<D, kRows<NARROW>>, dim3(ctas, NARROW ? 4 : 8), dim3(256), 0, s, a);
+    // 16 CTAs a cut block: all of its 128 rows at once, or half of 256 (4 and 8: a verify window 32.2 us, not 30.4)
+    return launch(join_k<D, kRows<NARROW>>, dim3(ctas, 16), dim3(256), 0, s, a);
 }
 
 }  // namespace
