@@ -459,7 +459,8 @@ size_t prompt_workspace(int d, int64_t rows) {
 }
 int prompt_launch(const b200q_paged& kv, const AttnArgs& a, void* stream) {
     const cudaStream_t s = (cudaStream_t)stream;
-    const bool narrow = (int64_t)a.max_rows * a.group <= kTile;   // one sequence of 16 x 4 rows, 16384 keys: 38 us, not 46
+    // 8 verify windows of 16 tokens x 7 heads over 6000 keys: narrow 38 us, with a second tile of no rows 46
+    const bool narrow = (int64_t)a.max_rows * a.group <= kTile;
     if (kv.d == 128) return status_from(narrow ? launch_prompt<128, true>(kv, a, s) : launch_prompt<128, false>(kv, a, s));
     return status_from(narrow ? launch_prompt<64, true>(kv, a, s) : launch_prompt<64, false>(kv, a, s));
 }
