@@ -271,15 +271,17 @@ struct KvLoader {
     __device__ __forceinline__ void block(const At& p, int from, int to) {
         const int lane = threadIdx.x & 31, piece = min(1 << a.page_log2, kKeys), pieces = kKeys / piece;
         const int* tab = a.s.table + p.b * a.s.ldt;
-        auto lookup = [&](int i) {   // lane l: piece l's page, INT_MIN where no row sees it
+        // lane l: whether some row sees piece l of step i (apart from its page's number, which may be anything), and its page
+        auto seen = [&](int i) {
             const int key = (p.s.u0 + i) * kKeys + lane * piece;
-            return i < to && lane < pieces && key < p.s.hi && key + piece > p.s.lo ? tab[key >> a.page_log2] : INT_MIN;
+            return i < to && lane < pieces && key < p.s.hi && key + piece > p.s.lo;
         };
+        auto lookup = [&](int i) { return seen(i) ? tab[((p.s.u0 + i) * kKeys + lane * piece) >> a.page_log2] : 0; };
         int next = lookup(from);
         for (int i = from; i < to && !dead; i++, o++) {
             int page = next;
             next = lookup(i + 1);
-            const bool live = page != INT_MIN;
+            const bool live = seen(i);
             if (live && (page < 0 || page >= a.pages)) { bad = true; page = a.pages; }   // TMA fills zeros
             const int st = o % NS, row = ((p.s.u0 + i) * kKeys + lane * piece) & ((1 << a.page_log2) - 1);
             const uint32_t bytes = __popc(__ballot_sync(~0u, live)) * piece * D * 2;
