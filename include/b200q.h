@@ -368,7 +368,8 @@ int b200q_kv_append(const b200q_paged* kv, const void* q, const void* k, const v
  * query head h
  *   out = sum_j p_j v_j / sum_j p_j,   p_j = exp(s_j),   s_j = scale q . k_j, or softcap tanh(scale q . k_j / softcap)
  * over the keys j of kv head h / (hq / hkv) with position - window < j <= position (window 0: all up to the position).
- * A row that sees no key gets zeros.  q [rows][hq][d] and out [rows][hq][d] bf16, rows ldq / ldo elements apart (multiples
+ * A row that sees no key gets zeros; a key that it does not see leaves it alone, whatever its value holds (infinities and NaN
+ * of later tokens among them).  q [rows][hq][d] and out [rows][hq][d] bf16, rows ldq / ldo elements apart (multiples
  * of 8), 16-byte aligned, not overlapping.  Scores, sums and accumulators are fp32; the probabilities are rounded to bf16
  * for the product with v.  scale > 0; softcap 0 (none) to 1e38, scale / softcap finite.
  * decode: up to 16 rows a sequence (one new token, or a verify window).  prompt: any number.  max_rows >= the rows of

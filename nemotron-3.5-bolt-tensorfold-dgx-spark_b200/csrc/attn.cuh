@@ -26,6 +26,8 @@ struct AttnArgs {
     bool whole;                // decode form: no row block is cut, so none is joined
     int window;                // keys a row sees at most (INT_MAX / 2: no window)
     void* ws;
+    const __nv_bfloat16 *kp, *vp;   // the cache as row_again (attn_line.cuh) reads it; the kernels' tiles come by tensor maps
+    int64_t k_stride, v_stride;
     // row / group for rows below 2^31: with 2^s >= group > 2^(s-1) and mul = floor(2^32 (2^s - group) / group) + 1, the quotient
     // is (floor(row mul / 2^32) + row) >> s (Granlund and Montgomery)
     __device__ __forceinline__ int token(int row) const { return (int)((__umulhi((uint32_t)row, group_mul) + (uint32_t)row) >> group_shift); }
@@ -99,6 +101,7 @@ inline AttnArgs attn_args(const b200q_paged& kv, const void* q, int64_t ldq, int
     }
     a.window = window > 0 && window < INT_MAX / 2 ? window : INT_MAX / 2;
     a.ws = ws;
+    a.kp = (const __nv_bfloat16*)kv.k_pages; a.vp = (const __nv_bfloat16*)kv.v_pages; a.k_stride = kv.k_stride; a.v_stride = kv.v_stride;
     return a;
 }
 

@@ -94,8 +94,15 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ bool consumers_any(bool mine) {
+    uint32_t any;
+    asm volatile("{ .reg .pred p, q; setp.ne.u32 p, %1, 0; barrier.cta.red.or.pred.aligned q, 1, 256, p; selp.u32 %0, 1, 0, q; }"
+                 : "=r"(any) : "r"((uint32_t)mine) : "memory");
+    return any != 0;
+}
 
-template <int D, int NT>
+// MANY: steps with several rows a sequence, which see different keys (row_again); without that code a single token is 1 % faster
+template <int D, int NT, bool MANY>
 __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
 attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, AttnArgs a) {
     using S = Shape<D, NT>;
@@ -352,6 +359,7 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
             return y;
         };
         float* slot = slots(a.ws) + ((size_t)blockIdx.x * 2 + (skip == 0 ? 1 : 0)) * kSlot<D, RB>;
+        float check = 0.f;   // NaN once a value on its way out is not finite
 #pragma unroll
         for (int pass = 0; pass < (S::kFrags + kJoin - 1) / kJoin; pass++) {
             if (pass) consumers_sync();
@@ -373,6 +381,7 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
                     v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
                 }
                 const int d0 = f / NT * 16, r0 = f % NT * 8;
+                if (MANY) check = fmaf(v.x + v.y + v.z + v.w, 0.f, check);
                 if (whole_block) {
                     const float l0 = row_sum(r0 + t * 2), l1 = row_sum(r0 + t * 2 + 1);
                     const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;   // no key seen: zeros
@@ -403,21 +412,44 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
                 d.cu0 = p.cu0; d.row0 = row0; d.nrows = rows; d.h = p.h;
             }
         }
+        if (MANY && p.s.p0 != p.s.p1 && __builtin_expect(consumers_any(check != 0.f), 0)) {   // rows of several tokens: see row_again
+#pragma unroll 1
+            for (int row = warp; row < rows; row += kWarps) {
+                float ref = 0.f;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    if (row == nt * 8 + t * 2) ref = m[nt][0];
+                    if (row == nt * 8 + t * 2 + 1) ref = m[nt][1];
+                }
+                ref = __shfl_sync(~0u, ref, (row & 7) >> 1);
+                const float l = row_sum(row);
+                if (!(l < INFINITY)) continue;   // its scores are no numbers
+                const int rr = row0 + row, tok = a.token(rr);
+                const int64_t of_head = (int64_t)(p.h * a.group + rr - tok * a.group) * D;
+                row_again<D>(a, p.s.lo, p.s.hi, a.s.table + p.b * a.s.ldt, p.h, p.len - p.r + tok, u0 * kUnit, (u0 + n) * kUnit,
+                             a.q + (p.cu0 + tok) * a.ldq + of_head, ref, l == 0.f ? 0.f : 1.f / l,
+                             whole_block ? a.out + (p.cu0 + tok) * a.ldo + of_head : nullptr, slot + row * D);
+            }
+        }
         at = p.end();
         if (at < end) p.advance(a, nrb);
     }
 }
 
-template <int D, int NT>
-cudaError_t launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& a, cudaStream_t s) {
+template <int D, int NT, bool MANY>
+cudaError_t launch_form(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& a, cudaStream_t s) {
     const size_t smem = Shape<D, NT>::kSmem;
     static SmemOptIn opted;
-    cudaError_t e = opted.allow((const void*)attn_rows_k<D, NT>, smem);
+    cudaError_t e = opted.allow((const void*)attn_rows_k<D, NT, MANY>, smem);
     if (e != cudaSuccess) return e;
     const int ctas = min(device_sms(), kMaxShares);
-    e = launch(attn_rows_k<D, NT>, dim3(ctas), dim3((kWarps + 1) * 32), smem, s, mk, mv, a);
+    e = launch(attn_rows_k<D, NT, MANY>, dim3(ctas), dim3((kWarps + 1) * 32), smem, s, mk, mv, a);
     if (e != cudaSuccess) return e;
     return a.whole ? e : launch(join_k<D, Shape<D, NT>::kRows>, dim3(ctas, NT), dim3(256), 0, s, a);
+}
+template <int D, int NT>
+cudaError_t launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& a, cudaStream_t s) {
+    return a.max_rows > 1 ? launch_form<D, NT, true>(mk, mv, a, s) : launch_form<D, NT, false>(mk, mv, a, s);
 }
 
 // Rows a kv head that this kernel takes.  From 17 on its accumulators are short of registers, and its S and PV products pay

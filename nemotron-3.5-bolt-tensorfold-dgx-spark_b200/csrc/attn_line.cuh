@@ -243,6 +243,90 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *(uint32_t*)&v;
 }
 
+// ---------------------------------------------------------------------------------------------------------
+// Infinite and NaN values.  The products multiply every value of a tile with every row's probability, and 0 times such a value
+// is NaN: the value of a later token of the row block, or of one that has left a row's window, spoils rows that do not see it.
+// (Values that no row of the block sees are cleared before; the rows of one token see the same keys.)  So where a result of rows
+// of several tokens is not finite, the columns that such a value spoilt are added up again, key by key, by a warp a row.  Found
+// by the size of the results on their way out, which costs 1 % of a step of several tokens; looking through the values instead,
+// by the MMA warp or an idle one, or a second walk over the share at its end, cost 2 to 15 %.
+// ---------------------------------------------------------------------------------------------------------
+// The row at `pos` with query q: of the keys key0 .. key1 - 1, the share's part of a block with keys lo .. hi - 1, those that it
+// sees.  The result lies in out (bf16, times inv, a whole block) or part (fp32), both by reference ref.  Columns that the row's own
+// scores, or values that it sees, make NaN stay as they are.  Lanes hold D / 32 columns each: short code, since code between
+// the loops costs time although it is not run.
+template <int D>
+__device__ __forceinline__ void row_again(const AttnArgs& a, int lo, int hi, const int* tab, int h, int pos, int key0, int key1,
+                                          const __nv_bfloat16* q, float ref, float inv, __nv_bfloat16* out, float* part) {
+    constexpr int V = D / 32, kAtOnce = 4;
+    const int lane = threadIdx.x & 31, d0 = lane * V;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int j = 0; j < V; j++) bad |= (uint32_t)!(fabsf(out ? __bfloat162float(out[d0 + j]) : part[d0 + j]) < INFINITY) << j;
+    if (!__any_sync(~0u, bad)) return;
+    auto load = [&](const __nv_bfloat16* pages, int64_t stride, int key, float (&x)[V]) {   // zeros where the table names no page
+        const int page = tab[key >> a.page_log2];
+        uint32_t w[V / 2] = {};
+        if (page >= 0 && page < a.pages) {
+            const __nv_bfloat16* at = pages + page * stride + (((int64_t)h << a.page_log2) + (key & ((1 << a.page_log2) - 1))) * D + d0;
+#pragma unroll
+            for (int j = 0; j < V / 2; j++) w[j] = ((const uint32_t*)at)[j];
+        }
+#pragma unroll
+        for (int j = 0; j < V; j++) x[j] = __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+    };
+    const int first = max(0, pos - a.window + 1);   // the row sees keys first .. pos
+    uint32_t taint = 0;                             // columns in which a key that it does not see holds such a value
+#pragma unroll 1
+    for (int k = max(lo, key0); k < min(hi, key1); k++) {
+        if (k >= first && k <= pos) k = pos;
+        else {
+            float v[V];
+            load(a.vp, a.v_stride, k, v);
+#pragma unroll
+            for (int j = 0; j < V; j++) taint |= (uint32_t)!(fabsf(v[j]) < INFINITY) << j;
+        }
+    }
+    bad &= taint;
+    float x[V], acc[V] = {};
+#pragma unroll
+    for (int j = 0; j < V; j++) x[j] = __bfloat162float(q[d0 + j]);
+    const float z = ref == -INFINITY ? 0.f : ref;
+    const int end = min(pos + 1, key1);
+#pragma unroll 1
+    for (int k0 = max(first, key0); k0 < end; k0 += kAtOnce) {
+        uint32_t left = bad;   // columns not NaN by a value that the row sees: those stay so
+#pragma unroll
+        for (int j = 0; j < V; j++) left &= ~((uint32_t)(acc[j] != acc[j]) << j);
+        if (!__any_sync(~0u, left)) return;
+        float k[kAtOnce][V], v[kAtOnce][V];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++) {
+            load(a.kp, a.k_stride, min(k0 + i, end - 1), k[i]);
+            load(a.vp, a.v_stride, min(k0 + i, end - 1), v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++) {
+            float y = 0.f;
+#pragma unroll
+            for (int j = 0; j < V; j++) y = fmaf(x[j], k[i][j], y);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) y += __shfl_xor_sync(~0u, y, o);
+            if (a.cap_in != 0.f) y = capped(y, a.cap_in);
+            const float p = __bfloat162float(__float2bfloat16_rn(ex2(fmaf(y, a.c, -z))));   // as the products take it
+            if (k0 + i < end)
+#pragma unroll
+                for (int j = 0; j < V; j++) acc[j] = fmaf(p, v[i][j], acc[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < V; j++)
+        if (bad >> j & 1) {
+            if (out) out[d0 + j] = __float2bfloat16_rn(acc[j] * inv);
+            else part[d0 + j] = acc[j];
+        }
+}
+
 // The row blocks that a share's end cut: partial 0 is the share's last, the others the first of the shares after it.
 // blockIdx.y takes every gridDim.y-th set of rows.  A row's partials are dealt to as many of the eight warps as rows leave
 // it, their sums added in warp order.

@@ -329,6 +329,7 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;   // no key seen: zeros
                 const long long place = (p.cu0 + tok) * a.ldo + (int64_t)(p.h * a.group + row0 + mrow - tok * a.group) * D;
                 float* slot = slots(a.ws) + ((size_t)share * 2 + (from == 0 ? 1 : 0)) * kSlot<D, ROWS>;
+                float top[4] = {};   // the largest sizes of the row's results
                 if (n > 0) {
                     if (!dead && !wait_for(odone + t * 8, ns - 1 & 1)) dead = true;
                     __syncwarp();
@@ -344,6 +345,10 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                     } else
 #pragma unroll
                         for (int j = 0; j < 64; j++) v[j / 32][j % 32] = 0;
+                    auto look = [&] {
+#pragma unroll
+                        for (int y = 0; y < 32; y++) top[y & 3] = max3(top[y & 3], fabsf(val(v[y / 16][y % 16 * 2])), fabsf(val(v[y / 16][y % 16 * 2 + 1])));
+                    };
                     if (NARROW) {
                         // [16 pieces of 4 columns][128 rows]: a warp's lanes side by side
                         float4* second = (float4*)(base + (sout - sq)) + row;
@@ -365,6 +370,7 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                             e[2] = __float_as_uint(fmaf(val(e[2]), mine, x.z));
                             e[3] = __float_as_uint(fmaf(val(e[3]), mine, x.w));
                         }
+                        look();
                         if (whole) {
                             if (row < rows)
 #pragma unroll
@@ -377,6 +383,7 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                             continue;
                         }
                     }
+                    if (!NARROW) look();
                     if (whole) {   // through shared memory, to whole lines in the stores
 #pragma unroll
                         for (int ch = 0; ch < 8; ch++) {
@@ -404,6 +411,21 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                             *(uint4*)(dst + y * 4) =
                                 make_uint4(v[y / 8][y % 8 * 4], v[y / 8][y % 8 * 4 + 1], v[y / 8][y % 8 * 4 + 2], v[y / 8][y % 8 * 4 + 3]);
                     }
+                }
+                if (p.s.p0 != p.s.p1 && (!NARROW || t == 0)) {   // rows of several tokens: see row_again
+                    const float most = max3(max3(top[0], top[1], top[2]), top[3], top[3]);
+                    unsigned todo = __ballot_sync(~0u, row < rows && !(most < INFINITY) && sum < INFINITY);   // else its scores are no numbers
+                    __syncwarp();
+                    if (__builtin_expect(todo != 0, 0))
+#pragma unroll 1
+                        for (; todo; todo &= todo - 1) {
+                            const int i = __ffs(todo) - 1, ri = quarter * 32 + i, rr = row0 + ri, tk = a.token(rr);
+                            const int64_t of_head = (int64_t)(p.h * a.group + rr - tk * a.group) * D;
+                            row_again<D>(a, p.s.lo, p.s.hi, a.s.table + p.b * a.s.ldt, p.h, p.len - p.r + tk, (p.s.u0 + from) * kKeys,
+                                         (p.s.u0 + to) * kKeys, a.q + (p.cu0 + tk) * a.ldq + of_head, __shfl_sync(~0u, ref, i),
+                                         __shfl_sync(~0u, inv, i), whole ? a.out + (p.cu0 + tk) * a.ldo + of_head : nullptr,
+                                         slot + (size_t)(NARROW ? ri : t * kTile + ri) * D);
+                        }
                 }
                 tc_fence_before();   // O has been read before this tile's next P is handed over
                 if (NARROW) asm volatile("barrier.cta.sync.aligned 1, 256;" ::: "memory");   // the shared places have been read
