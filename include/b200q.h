@@ -351,8 +351,9 @@ typedef struct b200q_paged {
 /* Append (libbolt: bolt_kernels.cu:1735, and the steps before it): for each of `rows` rows
  *   q_out = bf16(rotate(norm(q))),  k_pages[slot] = bf16(rotate(norm(k))),  v_pages[slot] = bf16(v)
  * q [rows][hq][d], k and v [rows][hkv][d], fp32 or bf16 (x_dtype), rows ldq / ldk / ldv elements apart (16-byte
- * multiples; the fused projection's output can be passed as it is), q_out [rows][hq][d] bf16, rows ldo apart; q_out may
- * be q itself.  hq = 0 with q and q_out NULL appends keys and values alone.
+ * multiples; the fused projection's output can be passed as it is), q_out [rows][hq][d] bf16, rows ldo apart.  q_out may
+ * be q itself where q is bf16 and ldo = ldq; any other overlap with q, k or v is refused (its rows may lie between theirs
+ * in one buffer, at one pitch).  hq = 0 with q and q_out NULL appends keys and values alone.
  * norm: x * rsqrt(mean(x^2) + eps) * w over each head, w = q_norm / k_norm [d] (norm_dtype fp32 or bf16), NULL: none.
  * rotate: the first `rope` values of a head (a multiple of 16, 0: none) in pairs (i, i + rope / 2), or (2i, 2i + 1) when
  * interleaved, by the angle position * inv_freq[i] (fp32 [rope / 2]).

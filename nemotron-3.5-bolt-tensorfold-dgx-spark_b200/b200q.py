@@ -644,7 +644,8 @@ def k_kv_append(q, k, v, k_pages, v_pages, table, lens, cu, inv_freq=None, inter
     q [rows][hq][d] (or None), k and v [rows][hkv][d]: fp32 or bf16, rows at any 16-byte pitch (views of the fused
     projection's output); k_pages / v_pages [pages][hkv][page][d] bf16; table [batch][width], lens [batch],
     cu [batch + 1] int32; inv_freq: fp32 [rope / 2], rotates the first `rope` values of each query and key head;
-    q_norm / k_norm [d]: weights of the RMS norm of each head.  -> q_out [rows][hq][d] bf16 (padding rows unwritten)"""
+    q_norm / k_norm [d]: weights of the RMS norm of each head.  -> q_out [rows][hq][d] bf16 (padding rows unwritten), which
+    may be q itself where q is bf16 and lies apart from q, k and v otherwise"""
     kv, dev, hkv, d, _ = _paged(k_pages, v_pages, table, lens, cu)
     dt = k.dtype if isinstance(k, torch.Tensor) else None
     if dt is not torch.float32 and dt is not torch.bfloat16:

@@ -219,6 +219,13 @@ extern "C" int b200q_kv_append(const b200q_paged* kv, const void* q, const void*
         !aligned(q_norm, 16) || !aligned(k_norm, 16))
         return B200Q_EINVAL;
     if (rows == 0) return B200Q_OK;
+    // a row's heads go to several warps and batches of loads: q_out may lie on q where every value replaces itself, and nowhere
+    // else on what is still to be read
+    const bool in_place = q_out == q && x_dtype == B200Q_BF16 && (ldo == ldq || rows == 1);
+    if (hq > 0 && ((!in_place && !rows_apart(q_out, ldo * 2, wq * 2, q, ldq * e, wq * e, rows)) ||
+                   !rows_apart(q_out, ldo * 2, wq * 2, k, ldk * e, wk * e, rows) ||
+                   !rows_apart(q_out, ldo * 2, wq * 2, v, ldv * e, wk * e, rows)))
+        return B200Q_EINVAL;
     AppendArgs a = {};
     a.q = q; a.k = k; a.v = v; a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.rows = rows; a.hq = hq; a.hkv = kv->hkv;
     a.kp = (__nv_bfloat16*)kv->k_pages; a.vp = (__nv_bfloat16*)kv->v_pages; a.k_stride = kv->k_stride; a.v_stride = kv->v_stride;

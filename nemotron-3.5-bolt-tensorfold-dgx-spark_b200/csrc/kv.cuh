@@ -32,6 +32,15 @@ inline bool kv_ok(const b200q_paged* p) {
            (int64_t)p->width * p->page <= (1 << 30) && p->batch > 0 && p->batch <= 4096 && p->k_stride >= one &&
            p->v_stride >= one && p->k_stride % 8 == 0 && p->v_stride % 8 == 0 && p->k_stride < far && p->v_stride < far;
 }
+// Whether n rows of wa bytes, pa apart, and n rows of wb bytes, pb apart, share no byte.  At one pitch the rows of each may lie
+// between those of the other, as views of one buffer do; at two pitches whole ranges are compared.
+inline bool rows_apart(const void* a, int64_t pa, int64_t wa, const void* b, int64_t pb, int64_t wb, int64_t n) {
+    const int64_t x = (int64_t)(uintptr_t)a, y = (int64_t)(uintptr_t)b;
+    if (n <= 0 || x + (n - 1) * pa + wa <= y || y + (n - 1) * pb + wb <= x) return true;
+    if (n == 1 || pa != pb) return false;
+    const int64_t at = ((y - x) % pa + pa) % pa;
+    return at >= wa && at + wb <= pa;
+}
 inline KvSeqs kv_seqs(const b200q_paged& p) { return {p.table, p.lens, p.cu, p.ldt, p.width, p.batch}; }
 
 }  // namespace b200q
