@@ -15,6 +15,7 @@
 // 8 x 8 transpose (movmatrix) each; P is rounded to bf16 there, V's type: 2^-8 at most on weights that are summed with
 // independent signs, below the output's own rounding.  m, the sum and O stay in fp32.
 #include "attn_line.cuh"
+#include "ring.cuh"
 #include "tcgen05.cuh"
 
 namespace b200q {
@@ -149,7 +150,7 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
         // (one lane for all took 170 ns a unit, the time of 8 KB at the full rate).  A unit's stage was last that of the
         // unit NS >= 16 before it, so no lane waits for what another lane of its eight has yet to issue.
         bool bad_page = false;
-        int issued = 0;
+        int issued = 0, tried = 0;   // behind the lane's last unit; the last whose place it waited for
         for (long long at = begin; at < end;) {
             const int skip = p.from(begin), n = p.to(end) - skip, u0 = p.s.u0 + skip;
             const int* tab = a.s.table + p.b * a.s.ldt;
@@ -162,9 +163,10 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
                 for (int k = 0; k < 32; k += kWarps) {
                     const int i = i0 + k + lane;
                     int page = __shfl_sync(~0u, mine, k + (lane & 7));
-                    const int o = ordinal + i, st = o % NS;
+                    const int o = ordinal + i, st = Ring<NS>::stage(o);
                     const bool live = lane < kWarps && i < n && !dead;
-                    if (live && !tc_mbar_wait(empty + st * 8, (o / NS & 1) ^ 1)) dead = true;
+                    if (live) tried = o;
+                    if (live && !tc_mbar_wait(empty + st * 8, Ring<NS>::parity(o) ^ 1)) dead = true;
                     __syncwarp();
                     if (live && !dead) {
                         if (page < 0 || page >= a.pages) { bad_page = true; page = a.pages; }   // past the end: TMA fills zeros
@@ -184,9 +186,18 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
         }
         if (dead && lane == 0) atomicOr(&g_attn_error, 1);
         if (__any_sync(~0u, bad_page) && lane == 0) atomicOr(&g_attn_error, 2);
-        // the last copies have landed before the block ends, whatever became of their readers
-        issued = __reduce_max_sync(~0u, issued);
-        for (int o = max(0, issued - NS) + lane; o < issued; o += 32) tc_mbar_wait(full + (o % NS) * 8, o / NS & 1);
+        // The last copy of every stage has landed before the block ends, whatever became of its readers.  Where a wait ran out, some
+        // of the last eight were issued and others not.
+        using R = Ring<NS>;
+        auto landed = [&](int o) { tc_mbar_wait(full + R::stage(o) * 8, R::parity(o)); };
+        if (!dead) {
+            issued = __reduce_max_sync(~0u, issued);
+            for (int o = R::oldest(issued) + lane; o < issued; o += 32) landed(o);
+        } else {
+            const int base = __shfl_sync(~0u, tried, 0), mine = R::last(base + lane, issued == base + lane + 1);
+            for (int o = max(0, base + kWarps - NS) + lane; o < base; o += 32) landed(o);
+            if (lane < kWarps && mine >= 0) landed(mine);
+        }
         return;
     }
 

@@ -2,6 +2,7 @@
 // and the softmax of 128 scores of a row held by one thread.
 #pragma once
 #include "attn_line.cuh"
+#include "ring.cuh"
 #include "tcgen05.cuh"
 
 namespace b200q {
@@ -265,7 +266,8 @@ struct KvLoader {
     uint32_t sk, sv, kfull, kempty, vfull, vempty;
     const CUtensorMap *mk, *mv;
     const AttnArgs& a;
-    int o = 0;               // steps so far
+    int o = 0;               // steps whose copies were issued
+    bool half = false;       // the wait for V's place ran out: of step o K's copies were issued
     bool dead = false, bad = false;
     // steps from .. to - 1 of the block at p
     __device__ __forceinline__ void block(const At& p, int from, int to) {
@@ -278,19 +280,19 @@ struct KvLoader {
         };
         auto lookup = [&](int i) { return seen(i) ? tab[((p.s.u0 + i) * kKeys + lane * piece) >> a.page_log2] : 0; };
         int next = lookup(from);
-        for (int i = from; i < to && !dead; i++, o++) {
+        for (int i = from; i < to; i++, o++) {
             int page = next;
             next = lookup(i + 1);
             const bool live = seen(i);
             if (live && (page < 0 || page >= a.pages)) { bad = true; page = a.pages; }   // TMA fills zeros
-            const int st = o % NS, row = ((p.s.u0 + i) * kKeys + lane * piece) & ((1 << a.page_log2) - 1);
+            const int st = Ring<NS>::stage(o), row = ((p.s.u0 + i) * kKeys + lane * piece) & ((1 << a.page_log2) - 1);
             const uint32_t bytes = __popc(__ballot_sync(~0u, live)) * piece * D * 2;
 #pragma unroll
             for (int side = 0; side < 2; side++) {
                 const uint32_t full = (side ? vfull : kfull) + st * 8;
-                if (!wait_for((side ? vempty : kempty) + st * 8, (o / NS & 1) ^ 1)) dead = true;
+                if (!wait_for((side ? vempty : kempty) + st * 8, Ring<NS>::parity(o) ^ 1)) dead = true;
                 dead = __any_sync(~0u, dead);
-                if (dead) break;
+                if (dead) { half = side == 1; return; }
                 if (lane == 0) tc_mbar_arrive_tx(full, bytes);
                 __syncwarp();
                 if (live)
@@ -301,15 +303,20 @@ struct KvLoader {
             }
         }
     }
-    // every stage's last release, and so every copy, has landed before the block ends
+    // every stage's last release, and so every copy, has landed before the block ends; where a wait ran out, every copy alone
     __device__ __forceinline__ void drain(int* error) {
+        using R = Ring<NS>;
         const int lane = threadIdx.x & 31;
         if (!dead)
-            for (int i = max(0, o - NS) + lane; i < o; i += 32)
-                if (!wait_for(kempty + (i % NS) * 8, i / NS & 1) || !wait_for(vempty + (i % NS) * 8, i / NS & 1)) dead = true;
-        if (dead)   // copies that were issued complete by themselves
-            for (int i = max(0, o + 1 - NS) + lane; i <= o; i += 32) { tc_mbar_wait(kfull + (i % NS) * 8, i / NS & 1); tc_mbar_wait(vfull + (i % NS) * 8, i / NS & 1); }
+            for (int i = R::oldest(o) + lane; i < o; i += 32)
+                if (!wait_for(kempty + R::stage(i) * 8, R::parity(i)) || !wait_for(vempty + R::stage(i) * 8, R::parity(i))) dead = true;
         dead = __any_sync(~0u, dead);
+        if (dead)
+#pragma unroll
+            for (int side = 0; side < 2; side++) {
+                const int issued = o + (half && side == 0);
+                for (int i = R::oldest(issued) + lane; i < issued; i += 32) wait_for((side ? vfull : kfull) + R::stage(i) * 8, R::parity(i));
+            }
         if (__any_sync(~0u, bad) && lane == 0) atomicOr(error, 2);
     }
 };
