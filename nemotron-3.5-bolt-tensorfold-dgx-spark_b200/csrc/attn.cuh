@@ -33,18 +33,14 @@ struct AttnArgs {
     __device__ __forceinline__ int token(int row) const { return (int)((__umulhi((uint32_t)row, group_mul) + (uint32_t)row) >> group_shift); }
 };
 
-// The exponent of a raw score q . k: with a cap, cap * tanh(scale q.k / cap) = cap * (1 - 2 / (exp(2 y) + 1)).  The
-// subtraction leaves 2^-23 of the cap, so below 2^-6 the series stands (its next term is 2^-26 of y); tanh.approx (2^-11)
-// would move a score of 50 by 0.02.
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float capped(float x, float cap_in) {
-    const float y = x * cap_in, t = 1.f - __fdividef(2.f, ex2(y * 2.885390081777927f) + 1.f);
-    return fabsf(y) < 0.015625f ? fmaf(y * y * y, -1.f / 3.f, y) : t;
-}
+// A raw score q . k with a cap, in caps: tanh(scale q.k / cap).  The exponent is the cap times it, so its relative error is the
+// score's: tanhf is within 2 steps throughout (1 - 2 / (exp(2 y) + 1) would leave 2^-23 of the cap, tanh.approx 2^-11).
+__device__ __forceinline__ float capped(float x, float cap_in) { return tanhf(x * cap_in); }
 
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap* m) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
@@ -92,10 +88,11 @@ inline AttnArgs attn_args(const b200q_paged& kv, const void* q, int64_t ldq, int
     a.c = 1.4426950408889634f * (softcap > 0.f ? softcap : scale);
     a.cap_in = softcap > 0.f ? scale / softcap : 0.f;
     // tanh(u) for |u| <= 3/8: u times the polynomial of degree 2 in u^2 with the least relative error (4.3e-6, a Remez fit), in
-    // terms of the score; its powers are ordinary numbers for scale / cap within 2^20 of 1
+    // terms of the score; its powers are ordinary numbers for scale / cap within 2^20 of 1.  Up to a capped score of 56 that is
+    // below 2^-12 of a probability, 2^-4 of P's rounding to bf16; beyond, as beyond 3/8 of the cap, tanhf.
     static const double tanh_poly[3] = {0.999995707885, -0.332780666598, 0.122647585951};
     if (a.cap_in > 0x1p-20f && a.cap_in < 0x1p20f) {
-        a.cap_near = 0.375f / a.cap_in;
+        a.cap_near = fminf(0.375f / a.cap_in, 56.f / scale);
         double u = a.cap_in;
         for (int k = 0; k < 3; k++, u *= (double)a.cap_in * a.cap_in) a.cap_poly[k] = (float)(tanh_poly[k] * u);
     }

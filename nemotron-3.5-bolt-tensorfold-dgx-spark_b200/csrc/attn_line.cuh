@@ -305,15 +305,22 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, int lo, int hi, con
             load(a.kp, a.k_stride, min(k0 + i, end - 1), k[i]);
             load(a.vp, a.v_stride, min(k0 + i, end - 1), v[i]);
         }
+        float y[kAtOnce], mine = 0.f;
 #pragma unroll
         for (int i = 0; i < kAtOnce; i++) {
-            float y = 0.f;
+            y[i] = 0.f;
 #pragma unroll
-            for (int j = 0; j < V; j++) y = fmaf(x[j], k[i][j], y);
+            for (int j = 0; j < V; j++) y[i] = fmaf(x[j], k[i][j], y[i]);
 #pragma unroll
-            for (int o = 16; o; o >>= 1) y += __shfl_xor_sync(~0u, y, o);
-            if (a.cap_in != 0.f) y = capped(y, a.cap_in);
-            const float p = __bfloat162float(__float2bfloat16_rn(ex2(fmaf(y, a.c, -z))));   // as the products take it
+            for (int o = 16; o; o >>= 1) y[i] += __shfl_xor_sync(~0u, y[i], o);
+            if (lane == i) mine = y[i];
+        }
+        // lane i: the probability of key i, as the products take it
+        if (a.cap_in != 0.f) mine = capped(mine, a.cap_in);
+        mine = __bfloat162float(__float2bfloat16_rn(ex2(fmaf(mine, a.c, -z))));
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++) {
+            const float p = __shfl_sync(~0u, mine, i);
             if (k0 + i < end)
 #pragma unroll
                 for (int j = 0; j < V; j++) acc[j] = fmaf(p, v[i][j], acc[j]);
