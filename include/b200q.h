@@ -372,7 +372,8 @@ int b200q_kv_append(const b200q_paged* kv, const void* q, const void* k, const v
  * A row that sees no key gets zeros; a key that it does not see leaves it alone, whatever its value holds (infinities and NaN
  * of later tokens among them).  q [rows][hq][d] and out [rows][hq][d] bf16, rows ldq / ldo elements apart (multiples
  * of 8), 16-byte aligned, not overlapping.  Scores, sums and accumulators are fp32; the probabilities are rounded to bf16
- * for the product with v.  scale > 0; softcap 0 (none) to 1e38, scale / softcap finite.
+ * for the product with v, and the prompt form takes the cap's tanh with an error below 2^-12 in the exponent.  0 < scale < 2e38;
+ * softcap 0 (none) or below 1e38 with scale / softcap an ordinary fp32 number (2^-126 at least, finite).
  * decode: up to 16 rows a sequence (one new token, or a verify window).  prompt: any number.  max_rows >= the rows of
  * every sequence (a sequence with more sets bit 22 of b200q_device_error, and some of its rows are left out).
  * A table entry outside the cache reads as zeros, a length outside 0 .. width * page is brought inside; both set bit 21.

@@ -1,6 +1,7 @@
 // Shared pieces of the paged attention kernels: their arguments, the score's scaling, the cache's tensor maps.
 #pragma once
 #include <atomic>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 
@@ -75,7 +76,8 @@ inline bool attn_ok(const b200q_paged* kv, const void* q, int64_t ldq, int rows,
     return kv_ok(kv) && q && out && workspace && aligned(q, 16) && aligned(out, 16) && aligned(workspace, 16) && ldq % 8 == 0 &&
            ldo % 8 == 0 && rows >= 0 && hq > 0 && hq <= 4096 && hq % kv->hkv == 0 && ldq >= (int64_t)hq * kv->d &&
            ldo >= (int64_t)hq * kv->d && max_rows > 0 && (int64_t)max_rows * (hq / kv->hkv) < (1 << 30) && scale > 0.f &&
-           scale < INFINITY && softcap >= 0.f && softcap < 1e38f && (softcap == 0.f || scale / softcap < INFINITY) && window >= 0;
+           scale < 2e38f && softcap >= 0.f && softcap < 1e38f &&   // the exponents' factor, log2 e times one of them, is finite
+           (softcap == 0.f || (scale / softcap < INFINITY && scale / softcap >= FLT_MIN)) && window >= 0;
 }
 inline AttnArgs attn_args(const b200q_paged& kv, const void* q, int64_t ldq, int rows, int hq, int max_rows, float scale, float softcap,
                           int window, void* out, int64_t ldo, void* ws) {
