@@ -16,10 +16,14 @@ import struct
 import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-# the library: B200Q_LIB if set (like libbolt's TENSORFOLD_BOLT_LIB lookup, bolt_api.zig:128-140), else the in-place build
-LIB_PATH = os.environ.get("B200Q_LIB") or os.path.join(HERE, "libb200q.so")
+# the library: B200Q_LIB if set (like libbolt's TENSORFOLD_BOLT_LIB lookup, bolt_api.zig:128-140), else the in-place build,
+# else what build.py could build without the IQ2_XXS tables
+PART = "libb200q_tablefree.so"
+LIB_PATH = os.environ.get("B200Q_LIB") or next(
+    (p for p in (os.path.join(HERE, n) for n in ("libb200q.so", PART)) if os.path.exists(p)), os.path.join(HERE, "libb200q.so"))
 
 OK, EINVAL, ENOSPACE, ECUDA = 0, -1, -2, -3
+EMISSING = -100   # this module's own: the operator is not in the library that was loaded
 F32, BF16 = 0, 1
 ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
 
@@ -29,10 +33,15 @@ _LIB = None
 class B200QError(RuntimeError):
     def __init__(self, status, what):
         self.status = status
-        msg = lib().b200q_strerror(status).decode()
+        msg = (f"not in {os.path.basename(LIB_PATH)}, which was built without the IQ2_XXS tables" if status == EMISSING
+               else lib().b200q_strerror(status).decode())
         if status == ECUDA:
             msg += f" (cudaError {lib().b200q_last_cuda_error()})"
         super().__init__(f"{what}: {msg}")
+
+
+def _missing(name, *args):
+    raise B200QError(EMISSING, name)
 
 
 def lib():
@@ -114,7 +123,10 @@ def lib():
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name, None)
-            if fn is None:   # a library built without the IQ2_XXS tables (build.py): calling the operator fails
+            if fn is None:
+                if os.path.basename(LIB_PATH) != PART:
+                    raise RuntimeError(f"{LIB_PATH} lacks {name}: it is not this version's, run build.py")
+                setattr(L, name, functools.partial(_missing, name))   # calling the operator raises
                 continue
             fn.restype, fn.argtypes = res, args
         _LIB = L
