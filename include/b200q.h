@@ -333,8 +333,9 @@ int b200q_moe_decode_noalloc(const void* x, const void* logits, const void* up, 
  * The step: a ragged batch of rows.  Sequence b has rows cu[b] .. cu[b + 1] - 1 and lens[b] cached tokens, the step's
  * own included, so its row i of r stands at position lens[b] - r + i; the token at position p lives in page
  * table[b * ldt + p / page], row p % page.  cu [batch + 1], lens [batch] and table [batch][ldt >= width] are int32 on the
- * device, read by the kernels alone: a captured graph follows their contents.  Rows outside cu[0] .. cu[batch] - 1
- * (padding) are neither read nor written.  batch <= 4096, width * page <= 2^30.
+ * device, read by the kernels alone: a captured graph follows their contents.  Every array of rows holds all `rows` of them.
+ * Those outside cu[0] .. cu[batch] - 1 (padding) are never written, and what they hold is of no matter, but the append may
+ * read them: its loads leave before a row's place is known.  batch <= 4096, width * page <= 2^30.
  * --------------------------------------------------------------------------------------------------------- */
 typedef struct b200q_paged {
     const void* k_pages;   /* bf16; written by b200q_kv_append alone */
