@@ -84,7 +84,7 @@ template <typename T, int D, bool INTERLEAVED>
 __global__ void __launch_bounds__(kAppendWarps * 32, 4) kv_append_k(AppendArgs a, int parts) {
     pdl_wait();
     constexpr int kLanes = D / 8, kHeads = 32 / kLanes, U = Raw<T>::kUnroll;   // lanes of a head, heads of a load
-    __shared__ float2 angles[kAppendWarps][D / 2];
+    __shared__ alignas(16) float2 angles[kAppendWarps][D / 2];   // read two at a time
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t task = (int64_t)blockIdx.x * kAppendWarps + warp;
     const int t = (int)(task / parts), part = (int)(task - (int64_t)t * parts);
