@@ -3,7 +3,7 @@
 // over the keys it sees, in one pass over the cache with the running maximum m and sum.
 //
 // Bound by HBM: every key and value a row sees is read once for all rows and query heads of its kv head.  32 heads of d 128
-// over 8: 64 sequences of up to 6000 keys 157 us, 6.3 TB/s; one of 262144 keys 162 us, 6.6 TB/s; one of 1000 keys 10 us.
+// over 8: 64 sequences of up to 6000 keys 157 us, 6.3 TB/s; one of 262144 keys 162 us, 6.6 TB/s; one of 1000 keys 10.3 us.
 //
 // Work is shared as attn_line.cuh says, in units of 16 keys (within one page, since pages hold 16 or more) and one row block
 // of 8 NT rows a kv head, a CTA an SM.  More than 16 rows a kv head are the tensor core's (attn_prompt.cu).
@@ -57,13 +57,13 @@ namespace {
 
 constexpr int kWarps = 8;                    // consumer warps
 constexpr int kUnit = 16;                    // keys a unit
-constexpr int kMinUnits = 16;                // a share is not smaller: two units a warp (one: 11.7 us for a short call, not 10.3)
+constexpr int kMinUnits = 16;                // a share is not smaller: two units a warp (one sequence of 1100 keys 10.1 us; 32: 11.7, 8: 9.5)
 
 template <int D, int NT>
 struct Shape {
     static constexpr int kRows = 8 * NT;                     // rows of a row block
     static constexpr int kBytes = kUnit * D * 4;             // a unit: K [D / 64][16][128 B], then V
-    // 128 KB: 5 % slower at 64 sequences of 6000 keys
+    // 128 KB: 64 sequences of up to 6000 keys 161.5 us, not 156.5
     static constexpr int kStages = 192 * 1024 / kBytes;
     // A warp meets its own stages only.  Otherwise one could wait for a stage's next fill before its last has landed, and a
     // wait for the parity after next returns at once.
@@ -102,7 +102,8 @@ __device__ __forceinline__ bool consumers_any(bool mine) {
     return any != 0;
 }
 
-// MANY: steps with several rows a sequence, which see different keys (row_again); without that code a single token is 1 % faster
+// MANY: steps with several rows a sequence, which see different keys (row_again); without that code a single token's step is up to
+// 1 % faster (one sequence of 1000 keys 10.3 us, not 10.4)
 template <int D, int NT, bool MANY>
 __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
 attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, AttnArgs a) {
@@ -464,14 +465,14 @@ cudaError_t launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const Attn
 }
 
 // Rows a kv head that this kernel takes.  From 17 on its accumulators are short of registers, and its S and PV products pay
-// for every eight rows; the tensor-core kernel's step costs the same up to 128.  32 query heads of d 128 over 4 kv heads, this
-// kernel (with 32 rows a block, as measured) against that: 32 sequences of 4096 keys, 2 rows each: 72 / 76 us; 3 rows: 145 / 76;
-// 16 rows: 477 / 86.  One of 512 keys: 16 / 26, 27 / 25, 33 / 35; d 64: 14 / 22, 18 / 22, 22 / 27.
+// for every eight rows; the tensor-core kernel's step costs the same up to 128.  16 rows a kv head, this kernel against that one:
+// d 128 over 4 kv heads, one sequence of 512 keys 9.8 / 16.4 us, 32 of 4096 54.7 / 67.2, 4 of 16384 34.1 / 40.4; over 8, 32 of 4096
+// 99.1 / 100.0; d 64 over 4: 7.8 / 12.4, 34.9 / 45.1, 23.0 / 28.9.
 constexpr int kMostRows = 16;
-// Where the page table holds no more keys a sequence, and there is a CTA for every block, blocks are not cut: a CTA then reads a
-// block's keys alone, but nothing is joined and the second launch is saved.  In a stream of calls, whole against cut, 32 heads of
-// d 128 over 8, one sequence: 500 keys 7.2 / 8.5 us, 1000 keys 10.3 / 10.0; 16 sequences: 9.1 / 13.2 and 15.4 / 20.1.  The host's
-// part of a call is 13.3 / 15.8.
+// Where the page table holds no more keys a sequence, and there are no more blocks than CTAs, blocks are not cut: a CTA then reads
+// a block's keys alone, but nothing is joined and the second launch is saved.  (Shares are not below kMinUnits then either:
+// blocks under 256 keys share CTAs.)  In a stream of calls, whole against cut, 32 heads of d 128 over 8, one sequence: 500 keys
+// 7.2 / 8.1 us, 1000 keys 10.3 / 9.9; 16 sequences: 9.0 / 13.3 and 15.0 / 19.9.  From Python a call is 13.3 / 15.8, the host's part.
 constexpr int kWholeKeys = 1024;
 bool few(int hq, int hkv, int max_rows) { return (int64_t)max_rows * (hq / hkv) <= kMostRows; }
 int row_tiles(int hq, int hkv, int max_rows) { return max_rows * (hq / hkv) <= 8 ? 1 : 2; }

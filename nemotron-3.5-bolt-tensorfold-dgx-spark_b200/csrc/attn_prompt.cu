@@ -12,15 +12,16 @@
 // Where no sequence has more than 128 rows a kv head (a verify window, a short chunk), a block is 128 rows and both tiles hold
 // them (narrow): one takes the even steps, the other the odd ones, and their sums are joined at the end.
 //
-// m is not the running maximum but a reference at most 2^8 below it: the quotient is the same for any reference that
-// neither overflows nor loses the largest terms, and O (in TMEM) is rescaled only when the maximum has outgrown the
-// reference by 2^8, a few times a row instead of every step.  Probabilities are then at most 2^8, a row's sum at most
-// 2^8 n.  P is rounded to bf16 (2^-8 relative at most) for the product with V; scores, sums and O stay in fp32.
+// m is not the running maximum but, as published for attention on these tensor cores, a reference at most 2^8 below it: the
+// quotient is the same for any reference that neither overflows nor loses the largest terms, and O (in TMEM) is rescaled only
+// when the maximum has outgrown the reference by 2^8, a few times a row instead of every step.  Probabilities are then at most
+// 2^8, a row's sum at most 2^8 n.  P is rounded to bf16 (2^-8 relative at most), the only type that multiplies V's; scores,
+// sums and O stay in fp32.
 //
 // Bound by each tile's chain: its exponentials, its PV, its next S.  8192 tokens of 32 heads over 8, d 128 (550 GFLOP): a step
 // of both tiles takes 3380 cycles, per tile 1500 for the exponentials (1024 of the special-function unit), 600 for the maximum
-// and its checks, 1140 from P to the next S; the tensor pipe works 2050 of them.  470 to 540 us as the power limit leaves
-// 1.4 to 1.6 GHz, 1020 to 1170 TFLOPS.
+// and its checks, 1140 from P to the next S; the tensor pipe works 2050 of them.  460 to 560 us as the power limit leaves
+// 1.4 to 1.6 GHz, 980 to 1190 TFLOPS.
 #include "attn_tc.cuh"
 
 namespace b200q {
@@ -46,7 +47,7 @@ template <bool NARROW>
 constexpr int kRows = NARROW ? kTile : 2 * kTile;
 constexpr int kThreads = 384;         // two softmax warpgroups; a MMA, a TMA and two Q warps
 constexpr int kOver = 2;              // what a row block costs besides its steps, in steps: its first and last step's waits
-constexpr int kMinShare = 1 + kOver;  // a share is not smaller, but for the division's rest: a block of one step (4: 77 tokens 16.8 us, not 13.3)
+constexpr int kMinShare = 1 + kOver;  // a share is not smaller, but for the division's rest: a block of one step (4: 77 tokens 14.5 us, not 10.8)
 
 template <int D>
 struct Lay {
@@ -468,9 +469,9 @@ cudaError_t launch_prompt(const b200q_paged& kv, const AttnArgs& a, cudaStream_t
     const int ctas = min(device_sms(), kMaxShares);
     e = launch(attn_prompt_k<D, NARROW>, dim3(ctas), dim3(kThreads), L::kSmem, s, mk, mv, a);
     if (e != cudaSuccess) return e;
-    // blocks of under four steps are not cut: nothing to join (77 tokens 12.6 -> 10.3 us)
+    // blocks of under four steps are not cut: nothing to join (77 tokens 10.8 us, with the launch 14.2)
     if ((int64_t)kv.width * kv.page <= 3 * kKeys) return e;
-    // 16 CTAs a cut block: all of its 128 rows at once, or half of 256 (4 and 8: a verify window 32.2 us, not 30.4)
+    // 16 CTAs a cut block: all of its 128 rows at once, or half of 256 (4: the verify window below 33.3 us, not 31.0; 8: 31.4)
     return launch(join_k<D, kRows<NARROW>>, dim3(ctas, 16), dim3(256), 0, s, a);
 }
 
@@ -481,7 +482,7 @@ size_t prompt_workspace(int d, int64_t rows) {
 }
 int prompt_launch(const b200q_paged& kv, const AttnArgs& a, void* stream) {
     const cudaStream_t s = (cudaStream_t)stream;
-    // 8 verify windows of 16 tokens x 7 heads over 6000 keys: narrow 38 us, with a second tile of no rows 46
+    // 8 verify windows of 16 tokens x 7 heads over 6000 keys: narrow 31 us, with a second tile of no rows 37
     const bool narrow = (int64_t)a.max_rows * a.group <= kTile;
     if (kv.d == 128) return status_from(narrow ? launch_prompt<128, true>(kv, a, s) : launch_prompt<128, false>(kv, a, s));
     return status_from(narrow ? launch_prompt<64, true>(kv, a, s) : launch_prompt<64, false>(kv, a, s));
