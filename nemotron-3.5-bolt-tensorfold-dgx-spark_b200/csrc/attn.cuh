@@ -22,6 +22,7 @@ struct AttnArgs {
     int pages, page_log2;
     float c;                   // a score times c is the exponent in powers of two (log2 e * scale; softcap: log2 e * cap)
     float cap_in;              // softcap: scale / cap, 0: none
+    bool cap_exact;            // a cap above 512
     float cap_near;            // scores up to here in size are capped by cap_poly: s sum_k cap_poly[k] s^2k (attn_tc.cuh)
     float cap_poly[3];
     bool whole;                // decode form: no row block is cut, so none is joined
@@ -39,9 +40,13 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// A raw score q . k with a cap, in caps: tanh(scale q.k / cap).  The exponent is the cap times it, so its relative error is the
-// score's: tanhf is within 2 steps throughout (1 - 2 / (exp(2 y) + 1) would leave 2^-23 of the cap, tanh.approx 2^-11).
-__device__ __forceinline__ float capped(float x, float cap_in) { return tanhf(x * cap_in); }
+// A raw score q . k with a cap, in caps: tanh(scale q.k / cap).  The exponent is the cap times it.  1 - 2 / (exp(2 y) + 1) leaves an
+// error of 1.5 2^-22 at most, below 2^-12 in the exponent for caps up to 512; from there on tanhf, right to 2 steps of its value
+// (it costs capped prompts a tenth more where scores come near the cap, so not for all; tanh.approx would leave 2^-11).
+__device__ __forceinline__ float capped(float x, float cap_in, bool exact) {
+    const float y = x * cap_in;
+    return exact ? tanhf(y) : 1.f - __fdividef(2.f, ex2(y * 2.885390081777927f) + 1.f);
+}
 
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap* m) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
@@ -89,9 +94,10 @@ inline AttnArgs attn_args(const b200q_paged& kv, const void* q, int64_t ldq, int
     a.pages = kv.pages; a.page_log2 = log2_of(kv.page);
     a.c = 1.4426950408889634f * (softcap > 0.f ? softcap : scale);
     a.cap_in = softcap > 0.f ? scale / softcap : 0.f;
+    a.cap_exact = softcap > 512.f;
     // tanh(u) for |u| <= 3/8: u times the polynomial of degree 2 in u^2 with the least relative error (4.3e-6, a Remez fit), in
     // terms of the score; its powers are ordinary numbers for scale / cap within 2^20 of 1.  Up to a capped score of 56 that is
-    // below 2^-12 of a probability, 2^-4 of P's rounding to bf16; beyond, as beyond 3/8 of the cap, tanhf.
+    // below 2^-12 of a probability, 2^-4 of P's rounding to bf16; beyond, as beyond 3/8 of the cap, capped().
     static const double tanh_poly[3] = {0.999995707885, -0.332780666598, 0.122647585951};
     if (a.cap_in > 0x1p-20f && a.cap_in < 0x1p20f) {
         a.cap_near = fminf(0.375f / a.cap_in, 56.f / scale);

@@ -292,9 +292,15 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
             float scale[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                if (a.cap_in != 0.f)
+                if (a.cap_in != 0.f) {
+                    if (a.cap_exact) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) s[nt][j] = capped(s[nt][j], a.cap_in);
+                        for (int j = 0; j < 4; j++) s[nt][j] = capped(s[nt][j], a.cap_in, true);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) s[nt][j] = capped(s[nt][j], a.cap_in, false);
+                    }
+                }
                 if (!whole)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {

@@ -316,7 +316,7 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, int lo, int hi, con
             if (lane == i) mine = y[i];
         }
         // lane i: the probability of key i, as the products take it
-        if (a.cap_in != 0.f) mine = capped(mine, a.cap_in);
+        if (a.cap_in != 0.f) mine = capped(mine, a.cap_in, a.cap_exact);
         mine = __bfloat162float(__float2bfloat16_rn(ex2(fmaf(mine, a.c, -z))));
 #pragma unroll
         for (int i = 0; i < kAtOnce; i++) {

@@ -142,8 +142,13 @@ __device__ __forceinline__ void cap_scores(Scores& s, uint32_t tmem_s, const Att
             uint32_t v[16];
             tmem_ld16(tmem_s + j * 16, v);
             tmem_ld_wait();
+            if (a.cap_exact) {
 #pragma unroll
-            for (int y = 0; y < 16; y++) v[y] = __float_as_uint(capped(val(v[y]), a.cap_in));
+                for (int y = 0; y < 16; y++) v[y] = __float_as_uint(capped(val(v[y]), a.cap_in, true));
+            } else {
+#pragma unroll
+                for (int y = 0; y < 16; y++) v[y] = __float_as_uint(capped(val(v[y]), a.cap_in, false));
+            }
             tmem_st16(tmem_s + j * 16, v);
         }
         tmem_st_wait();
