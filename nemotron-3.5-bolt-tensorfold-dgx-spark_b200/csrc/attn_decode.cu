@@ -430,25 +430,8 @@ attn_rows_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUte
                 d.cu0 = p.cu0; d.row0 = row0; d.nrows = rows; d.h = p.h;
             }
         }
-        if (MANY && p.s.p0 != p.s.p1 && __builtin_expect(consumers_any(check != 0.f), 0)) {   // rows of several tokens: see row_again
-#pragma unroll 1
-            for (int row = warp; row < rows; row += kWarps) {
-                float ref = 0.f;
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    if (row == nt * 8 + t * 2) ref = m[nt][0];
-                    if (row == nt * 8 + t * 2 + 1) ref = m[nt][1];
-                }
-                ref = __shfl_sync(~0u, ref, (row & 7) >> 1);
-                const float l = row_sum(row);
-                if (!(l < INFINITY)) continue;   // its scores are no numbers
-                const int rr = row0 + row, tok = a.token(rr);
-                const int64_t of_head = (int64_t)(p.h * a.group + rr - tok * a.group) * D;
-                row_again<D>(a, p.s.lo, p.s.hi, a.s.table + p.b * a.s.ldt, p.h, p.len - p.r + tok, u0 * kUnit, (u0 + n) * kUnit,
-                             a.q + (p.cu0 + tok) * a.ldq + of_head, ref, l == 0.f ? 0.f : 1.f / l,
-                             whole_block ? a.out + (p.cu0 + tok) * a.ldo + of_head : nullptr, slot + row * D);
-            }
-        }
+        // rows of several tokens: see row_again
+        if (MANY && p.s.p0 != p.s.p1 && __builtin_expect(consumers_any(check != 0.f), 0)) rows_again<D, RB, kUnit, 0, kWarps>(a, p, skip, skip + n, blockIdx.x);
         at = p.end();
         if (at < end) p.advance(a, nrb);
     }

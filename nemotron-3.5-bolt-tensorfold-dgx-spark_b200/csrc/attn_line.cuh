@@ -248,16 +248,17 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // is NaN: the value of a later token of the row block, or of one that has left a row's window, spoils rows that do not see it.
 // (Values that no row of the block sees are cleared before; the rows of one token see the same keys.)  So where a result of rows
 // of several tokens is not finite, the columns that such a value spoilt are added up again, key by key, by a warp a row.  Found
-// by the size of the results on their way out, which costs 1 % of a step of several tokens; looking through the values instead,
-// by the MMA warp or an idle one, or a second walk over the share at its end, cost 2 to 15 %.
+// by the size of the results on their way out; that and the code cost steps of several tokens 1 to 3 %, the shortest 5 (77 tokens
+// 10.6 -> 11.1 us).  Looking through the values instead, by the MMA warp or an idle one, cost 2 to 17 %.  A key takes a row 250 ns:
+// 8192 tokens of which the last holds NaN 54 ms, not 0.5.
 // ---------------------------------------------------------------------------------------------------------
 // The row at `pos` with query q: of the keys key0 .. key1 - 1, the share's part of a block with keys lo .. hi - 1, those that it
-// sees.  The result lies in out (bf16, times inv, a whole block) or part (fp32), both by reference ref.  Columns that the row's own
+// sees.  The result lies in out (bf16, a whole block) or part (fp32, a partial by reference ref).  Columns that the row's own
 // scores, or values that it sees, make NaN stay as they are.  Lanes hold D / 32 columns each: short code, since code between
 // the loops costs time although it is not run.
 template <int D>
 __device__ __forceinline__ void row_again(const AttnArgs& a, int lo, int hi, const int* tab, int h, int pos, int key0, int key1,
-                                          const __nv_bfloat16* q, float ref, float inv, __nv_bfloat16* out, float* part) {
+                                          const __nv_bfloat16* q, __nv_bfloat16* out, float* part, float ref) {
     constexpr int V = D / 32, kAtOnce = 4;
     const int lane = threadIdx.x & 31, d0 = lane * V;
     uint32_t bad = 0;
@@ -288,10 +289,9 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, int lo, int hi, con
         }
     }
     bad &= taint;
-    float x[V], acc[V] = {};
+    float x[V], acc[V] = {}, m = -INFINITY, sum = 0.f;   // sum: of every kAtOnce-th key, in the first lanes
 #pragma unroll
     for (int j = 0; j < V; j++) x[j] = __bfloat162float(q[d0 + j]);
-    const float z = ref == -INFINITY ? 0.f : ref;
     const int end = min(pos + 1, key1);
 #pragma unroll 1
     for (int k0 = max(first, key0); k0 < end; k0 += kAtOnce) {
@@ -299,39 +299,65 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, int lo, int hi, con
 #pragma unroll
         for (int j = 0; j < V; j++) left &= ~((uint32_t)(acc[j] != acc[j]) << j);
         if (!__any_sync(~0u, left)) return;
-        float k[kAtOnce][V], v[kAtOnce][V];
+        float k[kAtOnce][V], v[kAtOnce][V], mine = 0.f;
 #pragma unroll
         for (int i = 0; i < kAtOnce; i++) {
             load(a.kp, a.k_stride, min(k0 + i, end - 1), k[i]);
             load(a.vp, a.v_stride, min(k0 + i, end - 1), v[i]);
         }
-        float y[kAtOnce], mine = 0.f;
 #pragma unroll
         for (int i = 0; i < kAtOnce; i++) {
-            y[i] = 0.f;
+            float y = 0.f;
 #pragma unroll
-            for (int j = 0; j < V; j++) y[i] = fmaf(x[j], k[i][j], y[i]);
+            for (int j = 0; j < V; j++) y = fmaf(x[j], k[i][j], y);
 #pragma unroll
-            for (int o = 16; o; o >>= 1) y[i] += __shfl_xor_sync(~0u, y[i], o);
-            if (lane == i) mine = y[i];
+            for (int o = 16; o; o >>= 1) y += __shfl_xor_sync(~0u, y, o);
+            if (lane == i) mine = y;
         }
-        // lane i: the probability of key i, as the products take it
+        // lane i: key i's exponent and probability
         if (a.cap_in != 0.f) mine = capped(mine, a.cap_in, a.cap_exact);
-        mine = __bfloat162float(__float2bfloat16_rn(ex2(fmaf(mine, a.c, -z))));
+        mine = lane < kAtOnce && k0 + lane < end ? mine * a.c : -INFINITY;
+        float top = mine;
+#pragma unroll
+        for (int o = 1; o < kAtOnce; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+        top = fmaxf(m, __shfl_sync(~0u, top, 0));
+        const float z = top == -INFINITY ? 0.f : top, f = ex2(m - z), e = ex2(mine - z);
+        m = top;
+        sum = sum * f + e;
+#pragma unroll
+        for (int j = 0; j < V; j++) acc[j] *= f;
 #pragma unroll
         for (int i = 0; i < kAtOnce; i++) {
-            const float p = __shfl_sync(~0u, mine, i);
+            const float p = __bfloat162float(__float2bfloat16_rn(__shfl_sync(~0u, e, i)));   // as the products take it
             if (k0 + i < end)
 #pragma unroll
                 for (int j = 0; j < V; j++) acc[j] = fmaf(p, v[i][j], acc[j]);
         }
     }
 #pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    const float f = !out ? (m == -INFINITY ? 0.f : ex2(m - ref)) : sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
     for (int j = 0; j < V; j++)
         if (bad >> j & 1) {
-            if (out) out[d0 + j] = __float2bfloat16_rn(acc[j] * inv);
-            else part[d0 + j] = acc[j];
+            if (out) out[d0 + j] = __float2bfloat16_rn(acc[j] * f);
+            else part[d0 + j] = acc[j] * f;
         }
+}
+// Rows row, row + WARPS .. of the share's part of the block at p (units from .. to - 1), by this warp
+template <int D, int ROWS, int UNIT, int OVER, int WARPS>
+__device__ __forceinline__ void rows_again(const AttnArgs& a, const Cursor<ROWS, UNIT, OVER>& p, int from, int to, int share) {
+    const bool whole = from == 0 && to == p.s.n;
+    float* slot = slots(a.ws) + ((size_t)share * 2 + (from == 0 ? 1 : 0)) * kSlot<D, ROWS>;
+    const int row0 = p.rb * ROWS, rows = min(ROWS, p.r * a.group - row0);
+#pragma unroll 1
+    for (int row = threadIdx.x >> 5; row < rows; row += WARPS) {
+        const int rr = row0 + row, tok = a.token(rr);
+        const int64_t of_head = (int64_t)(p.h * a.group + rr - tok * a.group) * D;
+        row_again<D>(a, p.s.lo, p.s.hi, a.s.table + p.b * a.s.ldt, p.h, p.len - p.r + tok, (p.s.u0 + from) * UNIT, (p.s.u0 + to) * UNIT,
+                     a.q + (p.cu0 + tok) * a.ldq + of_head, whole ? a.out + (p.cu0 + tok) * a.ldo + of_head : nullptr, slot + row * D,
+                     whole ? 0.f : slot[ROWS * D + row]);
+    }
 }
 
 // The row blocks that a share's end cut: partial 0 is the share's last, the others the first of the shares after it.

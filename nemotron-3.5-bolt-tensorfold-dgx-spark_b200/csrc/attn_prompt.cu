@@ -55,7 +55,8 @@ struct Lay {
     static constexpr int kStages = D == 128 ? 2 : 4;          // of K and of V
     static constexpr int kOut = 8 * 32 * 128;                 // a warp's 32 rows of 64 columns on their way out
     static constexpr int kBars = 4 * kStages + 11;
-    static constexpr size_t kSmem = 1024 + (2 + 2 * kStages) * (size_t)kBytes + kOut + kBars * 8 + 16;
+    static constexpr int kFirst = 128;                        // the cursor at the share's start
+    static constexpr size_t kSmem = 1024 + (2 + 2 * kStages) * (size_t)kBytes + kOut + kBars * 8 + 16 + kFirst;
 };
 
 template <int D, bool NARROW>
@@ -89,6 +90,9 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
     const Shares split(total, shares);
     const long long begin = split.start(share), end = split.start(share + 1);
     At p = scan.seek(a, begin);
+    int* again = (int*)(base + (tslot - sq) + 4);   // whether a result is not finite
+    At* first = (At*)(base + (tslot - sq) + 16);
+    static_assert(sizeof(At) <= L::kFirst, "the cursor's place");
     // where tile t's rows begin among the sequence's (token, head) rows
     auto tile_row = [&](const At& c, int t) { return c.rb * ROWS + (NARROW ? 0 : t * kTile); };
     // tile t's part of steps from .. to - 1 of the block (counted from the block's first), as far as its rows see keys
@@ -118,6 +122,8 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
         tma_prefetch(&mk);
         tma_prefetch(&mv);
         desc[share].n = 0;   // unless the share ends inside a block, below
+        *first = p;
+        *again = 0;
     }
     if (warp == 8) tmem_take(tslot);
     tc_fence_before();
@@ -413,21 +419,8 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                                 make_uint4(v[y / 8][y % 8 * 4], v[y / 8][y % 8 * 4 + 1], v[y / 8][y % 8 * 4 + 2], v[y / 8][y % 8 * 4 + 3]);
                     }
                 }
-                if (p.s.p0 != p.s.p1 && (!NARROW || t == 0)) {   // rows of several tokens: see row_again
-                    const float most = max3(max3(top[0], top[1], top[2]), top[3], top[3]);
-                    unsigned todo = __ballot_sync(~0u, row < rows && !(most < INFINITY) && sum < INFINITY);   // else its scores are no numbers
-                    __syncwarp();
-                    if (__builtin_expect(todo != 0, 0))
-#pragma unroll 1
-                        for (; todo; todo &= todo - 1) {
-                            const int i = __ffs(todo) - 1, ri = quarter * 32 + i, rr = row0 + ri, tk = a.token(rr);
-                            const int64_t of_head = (int64_t)(p.h * a.group + rr - tk * a.group) * D;
-                            row_again<D>(a, p.s.lo, p.s.hi, a.s.table + p.b * a.s.ldt, p.h, p.len - p.r + tk, (p.s.u0 + from) * kKeys,
-                                         (p.s.u0 + to) * kKeys, a.q + (p.cu0 + tk) * a.ldq + of_head, __shfl_sync(~0u, ref, i),
-                                         __shfl_sync(~0u, inv, i), whole ? a.out + (p.cu0 + tk) * a.ldo + of_head : nullptr,
-                                         slot + (size_t)(NARROW ? ri : t * kTile + ri) * D);
-                        }
-                }
+                // rows of several tokens: see row_again
+                if (p.s.p0 != p.s.p1 && row < rows && !(max3(max3(top[0], top[1], top[2]), top[3], top[3]) < INFINITY)) *again = 1;
                 tc_fence_before();   // O has been read before this tile's next P is handed over
                 if (NARROW) asm volatile("barrier.cta.sync.aligned 1, 256;" ::: "memory");   // the shared places have been read
                 if (!whole) {
@@ -453,6 +446,15 @@ attn_prompt_k(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
     if (warp == 8) {
         tc_fence_after();
         tmem_free(tmem);
+    }
+    if (warp < 8 && *again) {   // the share's rows once more, here where no other warp's bounded wait is for these
+        p = *first;
+        for (;;) {
+            const int from = p.cut(begin), to = p.cut(end);
+            if (to > from && p.s.p0 != p.s.p1) rows_again<D, ROWS, kKeys, kOver, 8>(a, p, from, to, share);
+            if (p.end() >= end) break;
+            p.advance(a, nrb);
+        }
     }
 }
 

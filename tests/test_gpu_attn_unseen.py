@@ -122,3 +122,30 @@ def test_a_row_that_sees_an_infinity_keeps_it_beside_one_it_does_not_see():
             assert (out[:2, :, 9] == math.inf).all() and torch.isnan(out[2, :, 9]).all()
             out[:, :, 9] = 0
             assert torch.isfinite(out).all()
+
+
+def test_a_long_context_is_gone_over_without_another_warps_wait_running_out():
+    """262144 keys, the last token's value bad in every head: the block that holds its row has 255 more, each added up again over
+    all keys by a warp, which takes longer than the 2 s after which a wait of the block's other warps gives up"""
+    n, r, heads, d, page = 262144, 1280, 32, 64, 256
+    g = torch.Generator(device=DEV).manual_seed(0)
+    kp = torch.empty(n // page, heads, page, d, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    vp = torch.empty_like(kp).normal_(generator=g)
+    vp[-1, :, -1] = math.nan
+    q = torch.randn(r, heads, d, generator=g, device=DEV).bfloat16()
+    table = torch.arange(n // page, dtype=torch.int32, device=DEV)[None]
+    lens, cu = torch.tensor([n], dtype=torch.int32, device=DEV), torch.tensor([0, r], dtype=torch.int32, device=DEV)
+    out = b200q.attn_prompt(q, kp, vp, table, lens, cu, r)
+    torch.cuda.synchronize()
+    assert b200q.device_error() == 0
+    bad = torch.isnan(out.float())
+    assert bad[-1].all() and not bad[:-1].any()
+    for h in (0, 31):
+        k, v = kp[:, h].reshape(n, d).double(), vp[:, h].reshape(n, d).double()
+        for i in (r - 2, r - 100, r - 256, r - 257):
+            m = n - r + i + 1
+            p = torch.softmax(q[i, h].double() @ k[:m].T / 8, -1)
+            want, a = p @ v[:m], p @ v[:m].abs()
+            # p's rounding is off by 2^-8 a term at most, signs independent: 2^-8 of the norm of p v, which is the output's own
+            # for independent values; and the output's 2^-8.  A column with 1 / sqrt(n) of A is judged by the norm of all 64.
+            assert (out[i, h].double() - want).norm() <= 2.0 ** -6 * want.norm() and (want.abs() < 2.0 ** -4 * a).all()
