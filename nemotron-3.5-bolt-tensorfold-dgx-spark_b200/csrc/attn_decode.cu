@@ -455,13 +455,13 @@ cudaError_t launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const Attn
 
 // Rows a kv head that this kernel takes.  From 17 on its accumulators are short of registers, and its S and PV products pay
 // for every eight rows; the tensor-core kernel's step costs the same up to 128.  16 rows a kv head, this kernel against that one:
-// d 128 over 4 kv heads, one sequence of 512 keys 9.8 / 16.4 us, 32 of 4096 54.7 / 67.2, 4 of 16384 34.1 / 40.4; over 8, 32 of 4096
-// 99.1 / 100.0; d 64 over 4: 7.8 / 12.4, 34.9 / 45.1, 23.0 / 28.9.
+// d 128 over 4 kv heads, one sequence of 512 keys 9.7 / 16.7 us, 32 of 4096 55.0 / 63.6, 4 of 16384 34.1 / 38.3; over 8, 32 of 4096
+// 101 / 100; d 64 over 4: 7.7 / 13.1, 34.3 / 47.3, 22.6 / 29.1.
 constexpr int kMostRows = 16;
 // Where the page table holds no more keys a sequence, and there are no more blocks than CTAs, blocks are not cut: a CTA then reads
 // a block's keys alone, but nothing is joined and the second launch is saved.  (Shares are not below kMinUnits then either:
 // blocks under 256 keys share CTAs.)  In a stream of calls, whole against cut, 32 heads of d 128 over 8, one sequence: 500 keys
-// 7.2 / 8.1 us, 1000 keys 10.3 / 9.9; 16 sequences: 9.0 / 13.3 and 15.0 / 19.9.  From Python a call is 13.3 / 15.8, the host's part.
+// 7.2 / 8.1 us, 1000 keys 10.3 / 9.9; 16 sequences: 9.0 / 13.3 and 15.1 / 19.9.  From Python a call is 13.8 / 16, the host's part.
 constexpr int kWholeKeys = 1024;
 bool few(int hq, int hkv, int max_rows) { return (int64_t)max_rows * (hq / hkv) <= kMostRows; }
 int row_tiles(int hq, int hkv, int max_rows) { return max_rows * (hq / hkv) <= 8 ? 1 : 2; }

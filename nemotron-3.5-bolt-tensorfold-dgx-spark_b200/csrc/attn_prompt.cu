@@ -47,7 +47,7 @@ template <bool NARROW>
 constexpr int kRows = NARROW ? kTile : 2 * kTile;
 constexpr int kThreads = 384;         // two softmax warpgroups; a MMA, a TMA and two Q warps
 constexpr int kOver = 2;              // what a row block costs besides its steps, in steps: its first and last step's waits
-constexpr int kMinShare = 1 + kOver;  // a share is not smaller, but for the division's rest: a block of one step (4: 77 tokens 14.5 us, not 10.8)
+constexpr int kMinShare = 1 + kOver;  // a share is not smaller, but for the division's rest: a block of one step (4: 77 tokens 14.8 us, not 11.1)
 
 template <int D>
 struct Lay {
@@ -471,9 +471,9 @@ cudaError_t launch_prompt(const b200q_paged& kv, const AttnArgs& a, cudaStream_t
     const int ctas = min(device_sms(), kMaxShares);
     e = launch(attn_prompt_k<D, NARROW>, dim3(ctas), dim3(kThreads), L::kSmem, s, mk, mv, a);
     if (e != cudaSuccess) return e;
-    // blocks of under four steps are not cut: nothing to join (77 tokens 10.8 us, with the launch 14.2)
+    // blocks of under four steps are not cut: nothing to join (77 tokens 11.1 us, with the launch 14.4)
     if ((int64_t)kv.width * kv.page <= 3 * kKeys) return e;
-    // 16 CTAs a cut block: all of its 128 rows at once, or half of 256 (4: the verify window below 33.3 us, not 31.0; 8: 31.4)
+    // 16 CTAs a cut block: all of its 128 rows at once, or half of 256 (4: the verify window below 32.5 us, not 30.9; 8 as 16, ragged prompts 78.9, not 78.6)
     return launch(join_k<D, kRows<NARROW>>, dim3(ctas, 16), dim3(256), 0, s, a);
 }
 
@@ -484,7 +484,7 @@ size_t prompt_workspace(int d, int64_t rows) {
 }
 int prompt_launch(const b200q_paged& kv, const AttnArgs& a, void* stream) {
     const cudaStream_t s = (cudaStream_t)stream;
-    // 8 verify windows of 16 tokens x 7 heads over 6000 keys: narrow 31 us, with a second tile of no rows 37
+    // 8 verify windows of 16 tokens x 7 heads over 6000 keys: narrow 31 us, with a second tile of no rows 36
     const bool narrow = (int64_t)a.max_rows * a.group <= kTile;
     if (kv.d == 128) return status_from(narrow ? launch_prompt<128, true>(kv, a, s) : launch_prompt<128, false>(kv, a, s));
     return status_from(narrow ? launch_prompt<64, true>(kv, a, s) : launch_prompt<64, false>(kv, a, s));
